@@ -1,0 +1,558 @@
+// Attention of many new tokens over the engine's slot cache — gfx950 MFMA.
+//
+//   attn_prefill: packed prompts (or prompt chunks) of different lengths.
+//     Token i of sequence b sees the cache rows 0 .. start[b]+i of its slot:
+//     its history, the chunk's earlier tokens and itself (their K/V are in the
+//     cache already).
+//   attn_tree: N drafted tokens per sequence.  Node i sees the whole context
+//     (cache rows 0 .. ctx[b]-1) and, of the drafted nodes, its ancestors and
+//     itself; the drafts' K/V come in tensors of their own.
+//
+// Mathematics: out = softmax(scale * q K^T) V per (token, head), in one pass
+// over K/V with a running maximum m and sum l (both f32):
+//     m' = max(m, max_j s_j);  p_j = 2^((s_j - m') c),  c = scale * log2(e)
+//     l = l 2^((m-m') c) + sum p_j;  O = O 2^((m-m') c) + sum p_j v_j
+//
+// Layout: the G = heads / kv heads query heads of a kv head are packed with
+// the tokens into rows r = token * G + g, so K/V is read once per group.  Both
+// products run transposed on v_mfma_f32_32x32x16_bf16: S^T = K Q^T leaves lane
+// (h = lane/32, c = lane%32) with 16 scores of query row c, at key rows
+// 8b + 4h + i (b, i < 4).  The sum over keys in O^T = V^T P^T may run in any
+// order that both operands share, so these registers, rounded to bf16, ARE the
+// second product's B operand, and V^T is read from LDS to match
+// (ds_read_b64_tr_b16 gives a lane 4 consecutive key rows of one column).  P
+// never leaves the registers, and m, l and the rescaling are per lane.  P is
+// rounded to bf16 because the matrix cores take no wider second operand at
+// this rate: at most 2^-9 relative a weight, while l sums the f32 values.
+#include <hip/hip_runtime.h>
+#include <hip/hip_bf16.h>
+
+#include <cstdint>
+
+#define WAVE 64
+#define LOG2E 1.44269504088896340736f
+
+namespace {
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+
+struct AttnArgs {
+    const __hip_bfloat16* q;     // prefill [N, H, D]; tree [B, N, H, D]
+    __hip_bfloat16* out;         // as q
+    const void* k;               // [S, KVH, T, D] bf16 or e4m3
+    const void* v;
+    const __hip_bfloat16* k_new;  // tree: [B, N, KVH, D]
+    const __hip_bfloat16* v_new;
+    const int* slots;            // [B]
+    const int* ctx;              // [B] rows in the cache before the new tokens
+    const int* cu;               // prefill: [B + 1] first packed row of each sequence
+    const int* parents;          // tree: [B, N]
+    float* part_o;               // n_split > 1: [n_split, rows, H, D], unnormalised
+    float* part_ml;              // n_split > 1: [n_split, rows, H, 2]
+    long long q_sb, q_st, q_sh, o_sb, o_st, o_sh;        // strides in elements
+    long long k_ss, k_sh, k_st, v_ss, v_sh, v_st;
+    long long kn_sb, kn_st, kn_sh, vn_sb, vn_st, vn_sh;
+    int B, N, H, KVH, S, T, n_split;
+    float scale;
+};
+
+// max and sum over the two halves of a wave (lane and lane ^ 32)
+__device__ __forceinline__ float max_halves(float x) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_halves(float x) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ __forceinline__ unsigned fp8x2_to_bf16x2(unsigned w, bool hi) {
+    // e4m3 values are bf16 values: exact
+    bf16x2 r = hi ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true)
+                  : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false);
+    return __builtin_bit_cast(unsigned, r);
+}
+
+// Values of V that are not finite: all, +inf, -inf, NaN.
+enum Kind { BAD, PLUS, MINUS, NOT };
+// two bf16 in a word: all ones in the halves that hold that kind
+template <Kind K>
+__device__ __forceinline__ unsigned halves_where(unsigned w) {
+    const unsigned lo = w & 0xffffu, hi = w >> 16;
+    auto is = [](unsigned x) {
+        return K == BAD ? (x & 0x7f80u) == 0x7f80u : K == PLUS ? x == 0x7f80u : K == MINUS ? x == 0xff80u : (x & 0x7fffu) > 0x7f80u;
+    };
+    return (is(lo) ? 0xffffu : 0u) | (is(hi) ? 0xffff0000u : 0u);
+}
+// adds `value` to the accumulators whose row has a weight on a V of that kind
+template <Kind K>
+__device__ __forceinline__ f32x16 hits(u32x4 v, bf16x8 p) {
+    u32x4 one;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) one[i] = halves_where<K>(v[i]) & 0x3f803f80u;
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, one), p, (f32x16)0.f, 0, 0, 0);
+}
+template <Kind K>
+__device__ __forceinline__ void add_where(f32x16& acc, u32x4 v, bf16x8 p, float value) {
+    const f32x16 hit = hits<K>(v, p);
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        if (!(hit[i] == 0.f)) acc[i] += value;
+}
+
+// Tiles hold D bf16 a row in 16-byte chunks, permuted within the row so that
+// the reads below touch every bank once: 8 lanes reading one chunk column of 8
+// key rows (K), and 4 rows of 32 bytes, a pair of chunks (V).
+template <int D>
+__device__ __forceinline__ int k_chunk(int row, int c) {
+    return row * (D / 8) + (c ^ (row & (D / 8 - 1)));
+}
+template <int D>
+__device__ __forceinline__ int v_chunk(int row, int c) {
+    const int x = D == 128 ? (row & 7) << 1 : ((row >> 1) & 3) << 1;
+    return row * (D / 8) + (c ^ x);
+}
+
+// TREE: drafted nodes with their own K/V after the context.  KV8: e4m3 cache.
+// WR waves share the query rows of a tile (32 each), WK = 4 / WR split its keys.
+template <bool TREE, bool KV8, int D, int WR>
+__global__ void __launch_bounds__(256, 2) smg_attn_cache_t(AttnArgs a) {
+    constexpr int WK = 4 / WR;
+    constexpr int KB = WK == 4 ? 1 : 2;      // blocks of 32 keys a wave takes of a tile
+    constexpr int BN = 32 * KB * WK;         // keys of a tile
+    constexpr int BM = 32 * WR;              // query rows of a workgroup
+    constexpr int CPR = D / 8;               // 16-byte chunks a row
+    constexpr int HB = D / 32;
+    extern __shared__ u32x4 smem[];
+    u32x4* sk = smem;
+    u32x4* sv = smem + BN * CPR;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int wr = wave % WR, wk = wave / WR;
+    const int half = lane >> 5, col = lane & 31;
+    const int G = a.H / a.KVH;
+    const int kvh = blockIdx.x % a.KVH;
+    const int split = blockIdx.y;
+
+    // which sequence and rows: tiles of ceil(len * G / BM) a sequence
+    int b, row0, rows, base;  // base: first token of the sequence in q
+    if constexpr (TREE) {
+        const int per = (a.N * G + BM - 1) / BM;
+        const int tile = blockIdx.x / a.KVH;
+        b = tile / per;
+        row0 = (tile % per) * BM;
+        rows = a.N * G;
+        base = 0;
+    } else {
+        // the last tiles first: they see the most keys
+        int tile = gridDim.x / a.KVH - 1 - blockIdx.x / a.KVH;
+        b = -1;
+        row0 = rows = base = 0;
+        int before = 0;
+        for (int b0 = 0; b0 < a.B; b0 += WAVE) {
+            int lo = 0, hi = 0;
+            if (b0 + lane < a.B) {
+                lo = min(max(a.cu[b0 + lane], 0), a.N);
+                hi = min(max(a.cu[b0 + lane + 1], lo), a.N);
+            }
+            const int n = (int)(((long long)(hi - lo) * G + BM - 1) / BM);
+            int sum = n;
+#pragma unroll
+            for (int o = 1; o < WAVE; o <<= 1) {
+                const int up = __shfl_up(sum, o, WAVE);
+                if (lane >= o) sum += up;
+            }
+            const unsigned long long found = __ballot(before + sum > tile);
+            if (found) {
+                const int l = __ffsll((long long)found) - 1;
+                b = b0 + l;
+                base = __shfl(lo, l, WAVE);
+                rows = (__shfl(hi, l, WAVE) - base) * G;
+                row0 = (tile - before - __shfl(sum - n, l, WAVE)) * BM;
+                break;
+            }
+            before += __shfl(sum, WAVE - 1, WAVE);
+        }
+        if (b < 0) return;
+    }
+    const int slot = a.slots[b];
+    const bool cached = slot >= 0 && slot < a.S;
+    const int ctx = min(max(a.ctx[b], TREE ? 0 : -a.N), a.T);
+
+    // this lane's query row, and the last cache row that it sees
+    const int row = row0 + wr * 32 + col;
+    const bool live = row < rows;
+    const int token = min(row, rows - 1) / G;
+    const int head = kvh * G + min(row, rows - 1) % G;
+    const __hip_bfloat16* qp = a.q + (TREE ? b * a.q_sb : 0) + (base + token) * a.q_st + head * a.q_sh;
+    bf16x8 qf[D / 16];
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) qf[j] = *(const bf16x8*)(qp + j * 16 + half * 8);
+
+    int limit;                        // cache rows <= limit
+    unsigned long long nodes = 0;     // drafted nodes that this row sees
+    if constexpr (TREE) {
+        __shared__ int up[64];
+        __shared__ unsigned long long seen[64];
+        if (tid < a.N) up[tid] = a.parents[(size_t)b * a.N + tid];
+        __syncthreads();
+        if (tid < a.N) {
+            // a parent comes before its child, so the walk ends; anything else
+            // below -1 or not before it marks a node that is not in the tree
+            unsigned long long m = 0;
+            int i = tid;
+            while (i >= 0) {
+                m |= 1ull << i;
+                const int p = up[i];
+                if (p >= i || p < -1) {
+                    m = 0;
+                    break;
+                }
+                i = p;
+            }
+            seen[tid] = m;
+        }
+        __syncthreads();
+        nodes = live && cached ? seen[token] : 0;
+        limit = nodes ? ctx - 1 : -1;
+    } else {
+        limit = live && cached ? min(ctx + token, a.T - 1) : -1;
+    }
+
+    // keys of the workgroup, in tiles; a split takes a run of them
+    const int last_row = min(row0 + BM, rows) - 1;
+    const int kend = !cached ? 0 : TREE ? ctx : max(0, min(ctx + last_row / G + 1, a.T));
+    const int ctx_tiles = (kend + BN - 1) / BN;
+    const int new_tiles = TREE ? (a.N + BN - 1) / BN : 0;
+    const int tiles = ctx_tiles + (cached ? new_tiles : 0);
+    const int per_split = (tiles + a.n_split - 1) / a.n_split;
+    const int t0 = split * per_split, t1 = min(tiles, t0 + per_split);
+    const size_t unit = KV8 ? 1 : 2;
+    const char* kbase = (const char*)a.k + (cached ? slot * a.k_ss + kvh * a.k_sh : 0) * unit;
+    const char* vbase = (const char*)a.v + (cached ? slot * a.v_ss + kvh * a.v_sh : 0) * unit;
+    const __hip_bfloat16* knew = TREE ? a.k_new + b * a.kn_sb + kvh * a.kn_sh : nullptr;
+    const __hip_bfloat16* vnew = TREE ? a.v_new + b * a.vn_sb + kvh * a.vn_sh : nullptr;
+    const float c = a.scale * LOG2E;
+    // rows of this wave that see every key of a tile need no mask
+    int least = live ? limit : 0x7fffffff;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) least = min(least, __shfl_xor(least, o, WAVE));
+    least = __builtin_amdgcn_readfirstlane(least);
+
+    f32x16 acc[HB];
+#pragma unroll
+    for (int i = 0; i < HB; ++i) acc[i] = (f32x16)0.f;
+    float m = -INFINITY, l = 0.f;
+
+    for (int t = t0; t < t1; ++t) {
+        const bool fresh = TREE && t >= ctx_tiles;
+        const int n0 = fresh ? (t - ctx_tiles) * BN : t * BN;
+        const int nlast = (fresh ? a.N : kend) - 1;  // rows past the end repeat the last
+        __syncthreads();
+        for (int i = tid; i < BN * CPR; i += 256) {
+            const int r = i / CPR, cc = i % CPR;
+            const long long src = min(n0 + r, nlast);
+            u32x4 kx, vx;
+            if (KV8 && !fresh) {
+                const uint2 k8 = *(const uint2*)(kbase + src * a.k_st + cc * 8);
+                const uint2 v8 = *(const uint2*)(vbase + src * a.v_st + cc * 8);
+                kx = {fp8x2_to_bf16x2(k8.x, false), fp8x2_to_bf16x2(k8.x, true),
+                      fp8x2_to_bf16x2(k8.y, false), fp8x2_to_bf16x2(k8.y, true)};
+                vx = {fp8x2_to_bf16x2(v8.x, false), fp8x2_to_bf16x2(v8.x, true),
+                      fp8x2_to_bf16x2(v8.y, false), fp8x2_to_bf16x2(v8.y, true)};
+            } else {
+                const __hip_bfloat16* kr = fresh ? knew + src * a.kn_st : (const __hip_bfloat16*)kbase + src * a.k_st;
+                const __hip_bfloat16* vr = fresh ? vnew + src * a.vn_st : (const __hip_bfloat16*)vbase + src * a.v_st;
+                kx = *(const u32x4*)(kr + cc * 8);
+                vx = *(const u32x4*)(vr + cc * 8);
+            }
+            sk[k_chunk<D>(r, cc)] = kx;
+            sv[v_chunk<D>(r, cc)] = vx;
+        }
+        __syncthreads();
+
+        const int w0 = wk * KB * 32;  // this wave's keys of the tile
+        const bool masked = fresh || n0 + w0 + KB * 32 - 1 > least;  // the same in the whole wave
+        f32x16 s[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            s[kb] = (f32x16)0.f;
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) {
+                const bf16x8 kf = __builtin_bit_cast(bf16x8, sk[k_chunk<D>(w0 + kb * 32 + col, 2 * j + half)]);
+                s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[j], s[kb], 0, 0, 0);
+            }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if (masked) {
+                    const int key = n0 + w0 + kb * 32 + (i >> 2) * 8 + half * 4 + (i & 3);
+                    const bool sees = fresh ? (key < 64 && (nodes >> (key & 63) & 1)) : key <= limit;
+                    if (!sees) s[kb][i] = -INFINITY;
+                }
+                top = fmaxf(top, s[kb][i]);
+            }
+        top = max_halves(top);
+        const float m2 = fmaxf(m, top);
+        const float mc = m2 == -INFINITY ? 0.f : m2 * c;  // nothing seen yet: every p is 2^-inf
+        const float alpha = exp2f(m * c - mc);
+        m = m2;
+        l *= alpha;
+#pragma unroll
+        for (int i = 0; i < HB; ++i) acc[i] *= alpha;
+        bf16x8 p[KB][2];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float e = exp2f(fmaf(s[kb][i], c, -mc));
+                l += e;
+                p[kb][i >> 3][i & 7] = (__bf16)e;
+            }
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int hb = 0; hb < HB; ++hb) {
+                    // lane -> key rows r0 .. r0+3 (and r0+8 ..) of column hb*32 + col
+                    const int r0 = w0 + kb * 32 + j * 16 + half * 4 + ((lane & 15) >> 2);
+                    const int cc = hb * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+                    typedef __attribute__((address_space(3))) s16x4* lds_t;
+                    const char* lo = (const char*)&sv[v_chunk<D>(r0, cc)] + (lane & 1) * 8;
+                    const char* hi = (const char*)&sv[v_chunk<D>(r0 + 8, cc)] + (lane & 1) * 8;
+                    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)lo);
+                    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)hi);
+                    bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+                    if (masked) {
+                        // 0 * inf is NaN: a masked key's weight is 0, but its V must not
+                        // reach the rows that do not see it.  Such values are left out
+                        // here, and products of their own find the rows that they meet
+                        // with a weight.
+                        const u32x4 all = __builtin_bit_cast(u32x4, vf);
+                        u32x4 fin;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) fin[i] = all[i] & ~halves_where<BAD>(all[i]);
+                        vf = __builtin_bit_cast(bf16x8, fin);
+                        const u32x4 cut = fin ^ all;
+                        if (__any((cut[0] | cut[1] | cut[2] | cut[3]) != 0)) {
+                            add_where<PLUS>(acc[hb], all, p[kb][j], INFINITY);
+                            add_where<MINUS>(acc[hb], all, p[kb][j], -INFINITY);
+                            add_where<NOT>(acc[hb], all, p[kb][j], NAN);
+                        }
+                    }
+                    acc[hb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, p[kb][j], acc[hb], 0, 0, 0);
+                }
+    }
+    l = sum_halves(l);
+
+    // join the waves that took different keys: each finishes HB / WK of the columns
+    constexpr int HW = HB / WK;  // WK <= HB
+    if constexpr (WK > 1) {
+        float* so = (float*)smem;                     // [4][HB * 16][64]
+        float* sm = so + 4 * HB * 16 * WAVE;          // [4][2][64]
+        __syncthreads();
+#pragma unroll
+        for (int hb = 0; hb < HB; ++hb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) so[((wave * HB + hb) * 16 + i) * WAVE + lane] = acc[hb][i];
+        sm[(wave * 2) * WAVE + lane] = m;
+        sm[(wave * 2 + 1) * WAVE + lane] = l;
+        __syncthreads();
+        float f[WK], all = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < WK; ++w) all = fmaxf(all, sm[(wr + w * WR) * 2 * WAVE + lane]);
+#pragma unroll
+        for (int w = 0; w < WK; ++w) {
+            const float mw = sm[(wr + w * WR) * 2 * WAVE + lane];
+            f[w] = mw == -INFINITY ? 0.f : exp2f((mw - all) * c);
+            sum += f[w] * sm[((wr + w * WR) * 2 + 1) * WAVE + lane];
+        }
+        m = all;
+        l = sum;
+#pragma unroll
+        for (int hb = 0; hb < HW; ++hb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float o = 0.f;
+#pragma unroll
+                for (int w = 0; w < WK; ++w)
+                    o += f[w] * so[(((wr + w * WR) * HB + wk * HW + hb) * 16 + i) * WAVE + lane];
+                acc[hb][i] = o;
+            }
+    }
+    if (!live) return;
+    const int hb0 = WK > 1 ? wk * HW : 0;
+    if (a.n_split > 1) {
+        const size_t all_rows = (size_t)(TREE ? a.B * (long long)a.N : a.N);
+        const size_t at = ((size_t)split * all_rows + (TREE ? (size_t)b * a.N : base) + token) * a.H + head;
+#pragma unroll
+        for (int hb = 0; hb < HW; ++hb)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *(f32x4*)(a.part_o + at * D + (hb0 + hb) * 32 + j * 8 + half * 4) =
+                    (f32x4){acc[hb][j * 4], acc[hb][j * 4 + 1], acc[hb][j * 4 + 2], acc[hb][j * 4 + 3]};
+        if (wk == 0 && half == 0) {
+            a.part_ml[at * 2] = m;
+            a.part_ml[at * 2 + 1] = l;
+        }
+        return;
+    }
+    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // no key seen: zeros; NaN stays
+    __hip_bfloat16* op = a.out + (TREE ? b * a.o_sb : 0) + (base + token) * a.o_st + head * a.o_sh;
+#pragma unroll
+    for (int hb = 0; hb < HW; ++hb)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            bf16x4 o;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = (__bf16)(acc[hb][j * 4 + i] * inv);
+            *(bf16x4*)(op + (hb0 + hb) * 32 + j * 8 + half * 4) = o;
+        }
+}
+
+// Joins the splits of a row: out = sum_s 2^((m_s - m) c) O_s / sum_s 2^((m_s - m) c) l_s.
+// One wave a (token, head).
+template <bool TREE, int D>
+__global__ void __launch_bounds__(256) smg_attn_join_t(AttnArgs a) {
+    const int lane = threadIdx.x & 63;
+    const long long all_rows = TREE ? a.B * (long long)a.N : a.N;
+    const long long rh = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (rh >= all_rows * a.H) return;
+    const long long r = rh / a.H;
+    const int h = (int)(rh % a.H);
+    if constexpr (!TREE) {  // rows that no sequence covers stay as they are
+        if (r < max(a.cu[0], 0) || r >= a.cu[a.B]) return;
+    }
+    const float c = a.scale * LOG2E;
+    constexpr int E = D / WAVE;
+    float top = -INFINITY, sum = 0.f, o[E] = {};
+    for (int s = 0; s < a.n_split; ++s) top = fmaxf(top, a.part_ml[(s * all_rows * a.H + rh) * 2]);
+    for (int s = 0; s < a.n_split; ++s) {
+        const size_t at = s * all_rows * a.H + rh;
+        const float ms = a.part_ml[at * 2];
+        const float f = ms == -INFINITY ? 0.f : exp2f((ms - top) * c);
+        sum += f * a.part_ml[at * 2 + 1];
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] += f * a.part_o[at * D + lane * E + e];
+    }
+    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+    __hip_bfloat16* op = TREE ? a.out + r / a.N * a.o_sb + r % a.N * a.o_st : a.out + r * a.o_st;
+#pragma unroll
+    for (int e = 0; e < E; ++e) op[h * a.o_sh + lane * E + e] = (__hip_bfloat16)(o[e] * inv);
+}
+
+template <bool TREE, bool KV8, int D, int WR>
+int launch_t(const AttnArgs& a, hipStream_t s) {
+    constexpr int WK = 4 / WR, KB = WK == 4 ? 1 : 2, BM = 32 * WR;
+    constexpr int tile_bytes = 32 * KB * WK * D * 2 * 2;
+    constexpr int join_bytes = WK > 1 ? (4 * D / 32 * 16 * WAVE + 8 * WAVE) * 4 : 0;
+    constexpr int bytes = tile_bytes > join_bytes ? tile_bytes : join_bytes;
+    const long long G = a.H / a.KVH;
+    const long long tiles = TREE ? a.B * ((a.N * G + BM - 1) / BM) : a.N * G / BM + a.B;
+    const long long grid = tiles * a.KVH;
+    if (grid > 0x7fffffffll || a.n_split > 65535) return -5;
+    static bool set = false;  // more dynamic LDS than the default limit
+    if (!set) {
+        if (hipFuncSetAttribute((const void*)smg_attn_cache_t<TREE, KV8, D, WR>,
+                                hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
+            return -2;
+        set = true;
+    }
+    hipLaunchKernelGGL((smg_attn_cache_t<TREE, KV8, D, WR>), dim3((unsigned)grid, a.n_split), dim3(256), bytes, s, a);
+    if (a.n_split > 1) {
+        const long long rh = (TREE ? a.B * (long long)a.N : a.N) * a.H;
+        hipLaunchKernelGGL((smg_attn_join_t<TREE, D>), dim3((unsigned)((rh + 3) / 4)), dim3(256), 0, s, a);
+    }
+    return hipGetLastError() == hipSuccess ? 0 : -2;
+}
+
+template <bool TREE, bool KV8>
+int launch(const AttnArgs& a, int D, int wr, hipStream_t s) {
+    if (D == 128) {
+        if (wr == 1) return launch_t<TREE, KV8, 128, 1>(a, s);
+        if (wr == 2) return launch_t<TREE, KV8, 128, 2>(a, s);
+        return launch_t<TREE, KV8, 128, 4>(a, s);
+    }
+    if (D == 64) {
+        if (wr <= 2) return launch_t<TREE, KV8, 64, 2>(a, s);
+        return launch_t<TREE, KV8, 64, 4>(a, s);
+    }
+    return -1;
+}
+
+int bad_shape(int H, int KVH, int S, int T, int n_split) {
+    if (KVH <= 0 || H <= 0 || H % KVH) return -4;
+    if (S <= 0 || T <= 0 || n_split < 1) return -3;
+    return 0;
+}
+
+}  // namespace
+
+// strides: q token/head, out token/head, k slot/head/row, v slot/head/row
+extern "C" int smg_attn_prefill_launch(
+    const void* q, const void* k, const void* v, const void* slots, const void* ctx, const void* cu,
+    void* out, void* part_o, void* part_ml, const long long* strides, int B, int N, int H, int KVH,
+    int S, int T, int D, int n_split, int wr, float scale, int kv_fp8, void* stream) {
+    if (int rc = bad_shape(H, KVH, S, T, n_split)) return rc;
+    if (B < 1 || N < 1) return 0;
+    AttnArgs a = {};
+    a.q = (const __hip_bfloat16*)q;
+    a.out = (__hip_bfloat16*)out;
+    a.k = k;
+    a.v = v;
+    a.slots = (const int*)slots;
+    a.ctx = (const int*)ctx;
+    a.cu = (const int*)cu;
+    a.part_o = (float*)part_o;
+    a.part_ml = (float*)part_ml;
+    a.q_st = strides[0], a.q_sh = strides[1], a.o_st = strides[2], a.o_sh = strides[3];
+    a.k_ss = strides[4], a.k_sh = strides[5], a.k_st = strides[6];
+    a.v_ss = strides[7], a.v_sh = strides[8], a.v_st = strides[9];
+    a.B = B, a.N = N, a.H = H, a.KVH = KVH, a.S = S, a.T = T, a.n_split = n_split;
+    a.scale = scale;
+    return kv_fp8 ? launch<false, true>(a, D, wr, (hipStream_t)stream)
+                  : launch<false, false>(a, D, wr, (hipStream_t)stream);
+}
+
+// strides: q batch/token/head, out batch/token/head, k and v as above, k_new and v_new batch/token/head
+extern "C" int smg_attn_tree_launch(
+    const void* q, const void* k_new, const void* v_new, const void* k, const void* v,
+    const void* slots, const void* ctx, const void* parents, void* out, void* part_o, void* part_ml,
+    const long long* strides, int B, int N, int H, int KVH, int S, int T, int D, int n_split, int wr,
+    float scale, int kv_fp8, void* stream) {
+    if (int rc = bad_shape(H, KVH, S, T, n_split)) return rc;
+    if (N > 64) return -3;
+    if (B < 1 || N < 1) return 0;
+    AttnArgs a = {};
+    a.q = (const __hip_bfloat16*)q;
+    a.out = (__hip_bfloat16*)out;
+    a.k = k;
+    a.v = v;
+    a.k_new = (const __hip_bfloat16*)k_new;
+    a.v_new = (const __hip_bfloat16*)v_new;
+    a.slots = (const int*)slots;
+    a.ctx = (const int*)ctx;
+    a.parents = (const int*)parents;
+    a.part_o = (float*)part_o;
+    a.part_ml = (float*)part_ml;
+    a.q_sb = strides[0], a.q_st = strides[1], a.q_sh = strides[2];
+    a.o_sb = strides[3], a.o_st = strides[4], a.o_sh = strides[5];
+    a.k_ss = strides[6], a.k_sh = strides[7], a.k_st = strides[8];
+    a.v_ss = strides[9], a.v_sh = strides[10], a.v_st = strides[11];
+    a.kn_sb = strides[12], a.kn_st = strides[13], a.kn_sh = strides[14];
+    a.vn_sb = strides[15], a.vn_st = strides[16], a.vn_sh = strides[17];
+    a.B = B, a.N = N, a.H = H, a.KVH = KVH, a.S = S, a.T = T, a.n_split = n_split;
+    a.scale = scale;
+    return kv_fp8 ? launch<true, true>(a, D, wr, (hipStream_t)stream)
+                  : launch<true, false>(a, D, wr, (hipStream_t)stream);
+}

@@ -78,6 +78,26 @@ int smg_attn_decode_launch_split(const void* q, const void* k, const void* v, co
 int smg_attn_decode_launch_ex(const void* q, const void* k, const void* v, const void* pos,
                               void* out, int n_slots, int n_heads, int max_seq, int head_dim,
                               float scale, void* stream, int kv_fp8);
+// ---- attention of many new tokens over the slot cache (attn_cache.hip) ----
+int smg_attn_prefill_launch(const void* q, const void* k, const void* v, const void* slots,
+                            const void* ctx, const void* cu, void* out, void* part_o,
+                            void* part_ml, const long long* strides, int B, int N, int H, int KVH,
+                            int S, int T, int D, int n_split, int wr, float scale, int kv_fp8,
+                            void* stream);
+int smg_attn_tree_launch(const void* q, const void* k_new, const void* v_new, const void* k,
+                         const void* v, const void* slots, const void* ctx, const void* parents,
+                         void* out, void* part_o, void* part_ml, const long long* strides, int B,
+                         int N, int H, int KVH, int S, int T, int D, int n_split, int wr,
+                         float scale, int kv_fp8, void* stream);
+// ---- drafted tokens into the cache (tree_commit.hip) ----
+int smg_tree_commit_launch(const void* src, void* dst, const void* slots, const void* ctx,
+                           const void* parents, const void* tokens, const void* targets,
+                           void* count, void* path, void* next, const long long* strides, int B,
+                           int N, int L, int KVH, int S, int T, int D, int kv_fp8, void* stream);
+// ---- sampling (sample.hip) ----
+int smg_sample_launch(const void* logits, const void* u, const void* temperature,
+                      const void* top_k, const void* top_p, const void* min_p, void* out,
+                      long long stride, int R, int V, int f32, void* stream);
 // ---- fused decode elementwise (fused_decode.hip) ----
 int smg_rope_kv_store_launch(const void* qkv, const void* freqs, const void* pos,
                              void* k_cache, void* v_cache, void* q_out,
@@ -483,6 +503,77 @@ PYBIND11_MODULE(_core, m) {
               if (rc != 0) throw std::runtime_error("silu_mul launch failed rc=" + std::to_string(rc));
           },
           py::arg("gu"), py::arg("out"), py::arg("rows"), py::arg("inner"), py::arg("stream"));
+
+    // attention of many new tokens over the slot cache (attn_cache.hip);
+    // smg_amd/engine/ops.py checks the tensors and sizes the split
+    m.def("attn_prefill",
+          [](uintptr_t q, uintptr_t k, uintptr_t v, uintptr_t slots, uintptr_t ctx, uintptr_t cu,
+             uintptr_t out, uintptr_t part_o, uintptr_t part_ml, std::vector<long long> strides,
+             int B, int N, int H, int KVH, int S, int T, int D, int n_split, int wr, float scale,
+             int kv_fp8, uintptr_t stream) {
+              if (strides.size() != 10) throw std::runtime_error("attn_prefill takes 10 strides");
+              int rc = smg_attn_prefill_launch(
+                  (const void*)q, (const void*)k, (const void*)v, (const void*)slots,
+                  (const void*)ctx, (const void*)cu, (void*)out, (void*)part_o, (void*)part_ml,
+                  strides.data(), B, N, H, KVH, S, T, D, n_split, wr, scale, kv_fp8, (void*)stream);
+              if (rc != 0) throw std::runtime_error("attn_prefill launch failed rc=" + std::to_string(rc));
+          },
+          py::arg("q"), py::arg("k"), py::arg("v"), py::arg("slots"), py::arg("ctx"),
+          py::arg("cu"), py::arg("out"), py::arg("part_o"), py::arg("part_ml"), py::arg("strides"),
+          py::arg("B"), py::arg("N"), py::arg("H"), py::arg("KVH"), py::arg("S"), py::arg("T"),
+          py::arg("D"), py::arg("n_split"), py::arg("wr"), py::arg("scale"), py::arg("kv_fp8"),
+          py::arg("stream"));
+    m.def("attn_tree",
+          [](uintptr_t q, uintptr_t k_new, uintptr_t v_new, uintptr_t k, uintptr_t v,
+             uintptr_t slots, uintptr_t ctx, uintptr_t parents, uintptr_t out, uintptr_t part_o,
+             uintptr_t part_ml, std::vector<long long> strides, int B, int N, int H, int KVH, int S,
+             int T, int D, int n_split, int wr, float scale, int kv_fp8, uintptr_t stream) {
+              if (strides.size() != 18) throw std::runtime_error("attn_tree takes 18 strides");
+              int rc = smg_attn_tree_launch(
+                  (const void*)q, (const void*)k_new, (const void*)v_new, (const void*)k,
+                  (const void*)v, (const void*)slots, (const void*)ctx, (const void*)parents,
+                  (void*)out, (void*)part_o, (void*)part_ml, strides.data(), B, N, H, KVH, S, T, D,
+                  n_split, wr, scale, kv_fp8, (void*)stream);
+              if (rc != 0) throw std::runtime_error("attn_tree launch failed rc=" + std::to_string(rc));
+          },
+          py::arg("q"), py::arg("k_new"), py::arg("v_new"), py::arg("k"), py::arg("v"),
+          py::arg("slots"), py::arg("ctx"), py::arg("parents"), py::arg("out"), py::arg("part_o"),
+          py::arg("part_ml"), py::arg("strides"), py::arg("B"), py::arg("N"), py::arg("H"),
+          py::arg("KVH"), py::arg("S"), py::arg("T"), py::arg("D"), py::arg("n_split"),
+          py::arg("wr"), py::arg("scale"), py::arg("kv_fp8"), py::arg("stream"));
+    // accepted drafts into the cache (tree_commit.hip)
+    m.def("tree_commit",
+          [](uintptr_t src, uintptr_t dst, uintptr_t slots, uintptr_t ctx, uintptr_t parents,
+             uintptr_t tokens, uintptr_t targets, uintptr_t count, uintptr_t path, uintptr_t next,
+             std::vector<long long> strides, int B, int N, int L, int KVH, int S, int T, int D,
+             int kv_fp8, uintptr_t stream) {
+              if (strides.size() != 10) throw std::runtime_error("tree_commit takes 10 strides");
+              int rc = smg_tree_commit_launch(
+                  (const void*)src, (void*)dst, (const void*)slots, (const void*)ctx,
+                  (const void*)parents, (const void*)tokens, (const void*)targets, (void*)count,
+                  (void*)path, (void*)next, strides.data(), B, N, L, KVH, S, T, D, kv_fp8,
+                  (void*)stream);
+              if (rc != 0) throw std::runtime_error("tree_commit launch failed rc=" + std::to_string(rc));
+          },
+          py::arg("src"), py::arg("dst"), py::arg("slots"), py::arg("ctx"), py::arg("parents"),
+          py::arg("tokens"), py::arg("targets"), py::arg("count"), py::arg("path"),
+          py::arg("next"), py::arg("strides"), py::arg("B"), py::arg("N"), py::arg("L"),
+          py::arg("KVH"), py::arg("S"), py::arg("T"), py::arg("D"), py::arg("kv_fp8"),
+          py::arg("stream"));
+    // temperature / top-k / top-p / min-p sampling (sample.hip)
+    m.def("sample",
+          [](uintptr_t logits, uintptr_t u, uintptr_t temperature, uintptr_t top_k, uintptr_t top_p,
+             uintptr_t min_p, uintptr_t out, long long stride, int R, int V, int f32,
+             uintptr_t stream) {
+              int rc = smg_sample_launch((const void*)logits, (const void*)u,
+                                         (const void*)temperature, (const void*)top_k,
+                                         (const void*)top_p, (const void*)min_p, (void*)out, stride,
+                                         R, V, f32, (void*)stream);
+              if (rc != 0) throw std::runtime_error("sample launch failed rc=" + std::to_string(rc));
+          },
+          py::arg("logits"), py::arg("u"), py::arg("temperature"), py::arg("top_k"),
+          py::arg("top_p"), py::arg("min_p"), py::arg("out"), py::arg("stride"), py::arg("R"),
+          py::arg("V"), py::arg("f32"), py::arg("stream"));
 
     py::class_<PyHostTree>(m, "HostTokenTree")
         .def(py::init<uint32_t>(), py::arg("page_size") = 16)
