@@ -22,6 +22,7 @@ import torch
 _CACHE_TYPES = (torch.bfloat16, torch.float8_e4m3fn)
 HEAD_DIMS = (64, 128)
 MAX_NODES = 64
+MAX_VOCAB = 1 << 20
 
 
 def _core():
@@ -276,14 +277,14 @@ def sample(
     (float32 [R], 0 for none) of those the ones with w >= min_p; the first token of
     the order is always kept.  The answer is the first token by index at which the
     kept weights add up to more than u times their sum.  Weights count in multiples
-    of 2^-S, S = 62 - ceil(log2 V), in exact sums: the answer is the same every time,
+    of 2^-S, S = min(50, 62 - ceil(log2 V)), in exact sums: the answer is the same every time,
     and a token below half of that is never taken.  temperature (float32 [R]) 0
     takes the first token of the order.  -inf and NaN logits are never taken; a
     row of nothing else gives -1."""
     _check("logits", logits, (torch.bfloat16, torch.float32), 2)
     R, V = logits.shape
-    if V < 1:
-        raise ValueError("logits have no columns")
+    if not 1 <= V <= MAX_VOCAB:
+        raise ValueError(f"1 to {MAX_VOCAB} columns of logits, got {V}")
     if V > 1 and logits.stride(1) != 1:
         raise ValueError(f"logits must be dense in their last dimension, strides {logits.stride()}")
     dev = logits.device

@@ -456,7 +456,7 @@ def sample_plain(x, u, t, k=0, p=1.0, m=0.0):
         w = torch.exp((value - value[0]) / t)
         w[value == -math.inf] = 0
     n = max(1, int((w >= min(m, 1.0)).sum())) if m > 0 else V
-    unit = 2.0 ** (62 - (V - 1).bit_length())
+    unit = 2.0 ** min(50, 62 - (V - 1).bit_length())
     w = torch.floor(w * unit + 0.5) / unit
     if k > 0:
         w, index = w[:k], index[:k]
@@ -557,6 +557,31 @@ class TestSample:
         check_sample(x, US, 1.0, m=[0.0, -1.0, 1.0, 2.0, 1e-30, 0.999, 0.5, 0.3, 0.1])
         check_sample(x, [0.0, -1.0, 1.0, 2.0, 1e30, 0.5, 0.1, 0.2, 0.3], 1.0, k=100)
 
+    def test_far_off_logits(self):
+        # one value far below or above, as masks of the type's lowest value leave them
+        for V in (900, 40000):
+            x = randn(gen(7), len(US), V, dtype=torch.float32, scale=2.0)
+            x[:, 5] = -3.4e38
+            check_sample(x, US, math.inf, k=V // 2, p=0.7)
+            check_sample(x, US, 80.0, k=V - 2, p=0.7)
+            x[:, ::3] = torch.finfo(torch.float32).min
+            check_sample(x, US, 1.0, k=V // 2, p=0.9, m=0.01)
+            x[:, 11] = 3.4e38
+            check_sample(x, US, math.inf, k=9, p=0.7)
+            check_sample(x, US, 1.0, k=9, p=0.7)
+        x = randn(gen(8), len(US), 5000, dtype=torch.float32, scale=1e-42)  # denormals
+        check_sample(x, US, 1.0, k=100, p=0.5)
+
+    def test_many_values_within_one_step(self):
+        x = randn(gen(9), len(US), 30000, dtype=torch.float32, scale=1e-4)
+        x[:, 0] = 30.0
+        check_sample(x, US, 1.0, k=10000)
+        check_sample(x, US, 40.0, k=20000, p=0.6)
+
+    def test_largest_vocabulary(self):
+        x = randn(gen(10), 3, 1 << 20, scale=2.0)
+        check_sample(x, [0.3, 0.6, 0.999], 1.0, k=[0, 70000, 0], p=[1.0, 0.9, 0.95])
+
     def test_strides(self):
         g = gen(4)
         wide = randn(g, len(US), 5003)
@@ -656,6 +681,7 @@ class TestRefusals:
         ("sample", dict(logits=torch.zeros(2, 9, dtype=torch.float16)), TypeError),
         ("sample", dict(logits=torch.zeros(9)), ValueError),
         ("sample", dict(logits=torch.zeros(2, 0)), ValueError),
+        ("sample", dict(logits=torch.zeros(2, (1 << 20) + 1)), ValueError),
         ("sample", dict(logits=torch.zeros(9, 2).t()), ValueError),
         ("sample", dict(u=torch.zeros(3)), ValueError),
         ("sample", dict(u=torch.zeros(2, dtype=torch.float64)), TypeError),
