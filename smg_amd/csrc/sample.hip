@@ -17,9 +17,12 @@
 //
 // Both cuts are one search: the shortest prefix of the order whose measure (a
 // count, or a weight) reaches a number.  It runs over a histogram of NB equal
-// steps of the logit below the largest, which LDS atomics fill; the step in
-// which the number is reached is divided again, until it holds one value, and
-// equal values go by index.  Nothing is sorted.
+// steps of the logit below the largest, which LDS atomics fill.  The tokens of
+// the step in which the number is reached are compared with each other; where
+// they are more than CAND, the step is divided again, until it holds few tokens
+// or one value, and equal values go by index.  Nothing is sorted.  What a cut
+// leaves is listed in index order if it fits, and all that follows runs over the
+// list.
 //
 // A workgroup has a row, and each wave a run of it, 512 tokens at a time, 8 a
 // lane, so that index order is (wave, iteration, lane, element).
@@ -31,9 +34,9 @@
 #define WAVE 64
 #define THREADS 1024
 #define WAVES (THREADS / WAVE)
-#define NB 2048             // steps of a histogram; also the most blocks
+#define NB 2048             // steps of a histogram; also the most blocks and listed tokens
 #define BLOCK 512           // tokens of a wave's iteration
-#define HELD_ITS 4          // iterations that stay in registers: V <= 32768
+#define CAND 128            // tokens that are compared with each other
 #define MAX_V (NB * BLOCK)
 
 namespace {
@@ -55,43 +58,107 @@ struct SampleArgs {
 
 struct Shared {
     u64 hist[NB];
-    double pow2[64];  // 2^(i/64)
+    float list_x[NB];
+    int list_i[NB];
+    double pow2[64];  // 2^(i/64 + S)
     u64 part[WAVES];
     float lo[WAVES], hi[WAVES];
-    u64 above, total;
-    int bin, index;
+    int ints[WAVES];
+    u64 cand_m[CAND], cand_before[CAND];
+    float cand_x[CAND];
+    int cand_i[CAND];
+    u64 above;
+    float px;
+    int pi, bin, count, index;
 };
 
-template <typename T>
-__device__ __forceinline__ T wave_scan(T x) {  // inclusive
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < WAVE; o <<= 1) {
-        const T up = __shfl_up(x, o, WAVE);
-        if (lane >= o) x += up;
-    }
+// ---- a wave's scans, by lane moves within the vector unit ---------------------
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned moved(unsigned x, unsigned none) {
+    return (unsigned)__builtin_amdgcn_update_dpp((int)none, (int)x, CTRL, ROWS, 0xf, false);
+}
+// x of the lanes 1, 2, 4, 8 before within 16, then of lane 15 and lane 31 of the
+// 16s before: the six steps of an inclusive scan over 64 lanes
+#define SCAN_STEPS(STEP) STEP(0x111, 0xf) STEP(0x112, 0xf) STEP(0x114, 0xf) STEP(0x118, 0xf) STEP(0x142, 0xa) STEP(0x143, 0xc)
+
+__device__ __forceinline__ u64 wave_scan(u64 x) {
+#define STEP(CTRL, ROWS)                                                       \
+    x += (u64)moved<CTRL, ROWS>((unsigned)(x >> 32), 0) << 32 | moved<CTRL, ROWS>((unsigned)x, 0);
+    SCAN_STEPS(STEP)
+#undef STEP
     return x;
 }
+__device__ __forceinline__ int wave_scan(int x) {
+#define STEP(CTRL, ROWS) x += (int)moved<CTRL, ROWS>((unsigned)x, 0);
+    SCAN_STEPS(STEP)
+#undef STEP
+    return x;
+}
+__device__ __forceinline__ float wave_max(float x) {
+#define STEP(CTRL, ROWS) \
+    x = fmaxf(x, __uint_as_float(moved<CTRL, ROWS>(__float_as_uint(x), 0xff800000u)));
+    SCAN_STEPS(STEP)
+#undef STEP
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), 63));
+}
+__device__ __forceinline__ u64 at_lane(u64 x, int lane) {
+    return (u64)(unsigned)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32 |
+           (unsigned)__builtin_amdgcn_readlane((int)x, lane);
+}
+__device__ __forceinline__ u64 wave_sum(u64 x) { return at_lane(wave_scan(x), 63); }
 
-// Sums the NB counters of sh.hist; sh.bin and sh.above get the first at which
-// the sum reaches `want` and the sum before it (bin NB if it never does).
-__device__ __forceinline__ void locate(Shared& sh, u64 want) {
-    const int t = threadIdx.x, wave = t / WAVE;
+// (lowest, highest) over the workgroup
+__device__ __forceinline__ float2 block_range(Shared& sh, float lo, float hi) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / WAVE;
+    lo = wave_max(-lo), hi = wave_max(hi);
+    __syncthreads();
+    if (lane == 0) sh.lo[wave] = lo, sh.hi[wave] = hi;
+    __syncthreads();
+    lo = sh.lo[lane & (WAVES - 1)], hi = sh.hi[lane & (WAVES - 1)];
+    return make_float2(-wave_max(lo), wave_max(hi));
+}
+// the sum over the waves before this one of what each has in v[wave]
+template <typename T>
+__device__ __forceinline__ T before_wave(const T* v, T* all) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+    const T run = wave_scan(lane < WAVES ? v[lane] : (T)0);
+    if constexpr (sizeof(T) == 8) {
+        *all = at_lane(run, WAVES - 1);
+        return wave ? at_lane(run, wave - 1) : 0;
+    } else {
+        *all = __builtin_amdgcn_readlane(run, WAVES - 1);
+        return wave ? __builtin_amdgcn_readlane(run, wave - 1) : 0;
+    }
+}
+
+__device__ __forceinline__ void clear(Shared& sh) {
+    __syncthreads();
+    sh.hist[threadIdx.x] = sh.hist[threadIdx.x + THREADS] = 0;
+    __syncthreads();
+}
+
+// Adds the NB counters of sh.hist up: sh.bin and sh.above get the first at which
+// the sum reaches want(sum of all) and the sum before it (bin NB if it never
+// does).  Returns that want.
+template <typename W>
+__device__ __forceinline__ u64 locate(Shared& sh, W&& want_of) {
+    const int t = threadIdx.x;
     __syncthreads();
     const u64 a = sh.hist[2 * t], s = a + sh.hist[2 * t + 1];
     const u64 run = wave_scan(s);
-    if ((t & 63) == 63) sh.part[wave] = run;
+    if ((t & 63) == 63) sh.part[t / WAVE] = run;
     if (t == 0) sh.bin = NB;
     __syncthreads();
-    u64 before = run - s;
-    for (int w = 0; w < wave; ++w) before += sh.part[w];
+    u64 all;
+    const u64 before = before_wave(sh.part, &all) + run - s;
+    const u64 want = want_of(all);
     if (before < want && before + s >= want) {
         const bool second = before + a < want;
         sh.bin = 2 * t + second;
         sh.above = before + (second ? a : 0);
     }
-    if (t == THREADS - 1) sh.total = before + s;
     __syncthreads();
+    return want;
 }
 
 // the order's tokens up to the value x, of those equal to x up to index i
@@ -102,223 +169,301 @@ struct Prefix {
 };
 
 // exp((x - top) / t) in 64 bits: 2^(n/64) from a table times a polynomial of
-// 2^r, |r| <= 1/128 (off by 4e-14 at most)
+// 2^r, |r| <= 1/128 (off by 4e-14 at most), as a multiple of 2^-S
 struct Weigh {
     const double* pow2;
-    double top, c, magic;
-    int S;
+    double top, c, units;
+    float floor;  // below it weights are 0
     __device__ __forceinline__ void init(Shared& sh, float largest, float t, int V) {
+        const int S = min(50, 62 - (V > 1 ? 32 - __clz(V - 1) : 0));
+        units = (double)(1ull << S);
         pow2 = sh.pow2;
         top = (double)largest;
         c = 64. * 1.44269504088896340736 / (double)t;
-        S = min(50, 62 - (V > 1 ? 32 - __clz(V - 1) : 0));
+        floor = fmaxf(largest - 45.f * t, -3.40282347e38f);  // 2^-64
+        if (threadIdx.x < 64) sh.pow2[threadIdx.x] = exp2((double)threadIdx.x / 64) * units;
     }
-    __device__ __forceinline__ double mantissa(float x, int& e) const {
-        // -inf and NaN: weight 0
-        const double y = fmax(((double)x - top) * c, -1e9);
-        const double n = rint(y), r = y - n;
-        const int k = (int)n;
-        constexpr double q = 0.6931471805599453094 / 64;
+    __device__ __forceinline__ double scaled(float x) const {  // weight * 2^S
+        constexpr double magic = 6755399441055744., q = 0.6931471805599453094 / 64;
+        const double d = (double)fmaxf(x, floor) - top;  // NaN and -inf too go to the floor
+        const double n = fma(d, c, magic);  // the nearest integer in its low bits
+        const double r = fma(d, c, magic - n);
         double p = fma(r, q * q * q * q / 24, q * q * q / 6);
         p = fma(r, p, q * q / 2);
         p = fma(r, p, q);
         p = fma(r, p, 1.);
-        e = k >> 6;
-        return p * pow2[k & 63];
-    }
-    __device__ __forceinline__ double value(float x) const {
-        int e;
-        const double m = mantissa(x, e);
-        return ldexp(m, e);
+        const int k = (int)__double_as_longlong(n);
+        const long long bits = __double_as_longlong(p * pow2[k & 63]);
+        // times 2^(k/64): to the exponent, which stays in range (above 2^-66)
+        return __longlong_as_double(bits + ((long long)(k & ~63) << 46));
     }
     __device__ __forceinline__ u64 fixed(float x) const {
-        int e;
-        const double m = mantissa(x, e);
-        return (u64)__double_as_longlong(ldexp(m, e + S) + 4503599627370496.) & 0xfffffffffffffull;
+        const u64 w = (u64)__double_as_longlong(scaled(x) + 4503599627370496.) & 0xfffffffffffffull;
+        return x >= floor ? w : 0;
     }
 };
 
-// A row's tokens: `f(i, x)` for each of the thread's, in index order.
-template <bool F32, bool HELD>
+// ---- the tokens: f(i, x) for each of the thread's, in index order ---------------
+template <bool F32>
 struct Row {
     const char* at;
     int V, start, its, lane;
     bool infinite;  // the largest is +inf: those weigh 1, all others nothing
-    u32x4 raw[HELD ? HELD_ITS * (F32 ? 2 : 1) : 1];
 
-    __device__ __forceinline__ void load8(int it, u32x4* r) const {
+    struct Raw {
+        u32x4 w[F32 ? 2 : 1];
+    };
+    __device__ __forceinline__ Raw load8(int it) const {
         const int i = start + it * BLOCK + lane * 8;
+        Raw r;
         if (i + 8 <= V) {
             // rows may start anywhere: the hardware takes wide loads at any element
-            __builtin_memcpy(r, at + (size_t)i * (F32 ? 4 : 2), F32 ? 32 : 16);
+            __builtin_memcpy(&r, at + (size_t)i * (F32 ? 4 : 2), F32 ? 32 : 16);
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 if (F32)
-                    r[e / 4][e % 4] = i + e < V ? ((const unsigned*)at)[i + e] : 0x7fc00000u;
+                    r.w[e / 4][e % 4] = i + e < V ? ((const unsigned*)at)[i + e] : 0x7fc00000u;
                 else {
                     const unsigned h = i + e < V ? ((const unsigned short*)at)[i + e] : 0x7fc0u;
-                    r[0][e / 2] = e % 2 ? r[0][e / 2] | h << 16 : h;
+                    r.w[0][e / 2] = e % 2 ? r.w[0][e / 2] | h << 16 : h;
                 }
             }
         }
+        return r;
     }
     __device__ __forceinline__ void init(const SampleArgs& a) {
         lane = threadIdx.x & 63;
         V = a.V;
         at = (const char*)a.logits + blockIdx.x * a.stride * (F32 ? 4 : 2);
         its = (V + WAVES * BLOCK - 1) / (WAVES * BLOCK);
-        start = threadIdx.x / WAVE * its * BLOCK;
+        start = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE) * its * BLOCK;
         infinite = false;
-        if constexpr (HELD) {
-#pragma unroll
-            for (int it = 0; it < HELD_ITS; ++it) load8(it, raw + it * (F32 ? 2 : 1));
-        }
     }
     template <typename F>
-    __device__ __forceinline__ void each8(int it, F&& f) const {
-        u32x4 tmp[F32 ? 2 : 1];
-        const u32x4* r = tmp;
-        if constexpr (HELD)
-            r = raw + it * (F32 ? 2 : 1);
-        else
-            load8(it, tmp);
+    __device__ __forceinline__ void each8(int it, const Raw& r, F&& f) const {
         const int i = start + it * BLOCK + lane * 8;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            float x = __uint_as_float(F32 ? r[e / 4][e % 4] : e % 2 ? r[0][e / 2] & 0xffff0000u : r[0][e / 2] << 16);
+            float x = __uint_as_float(F32 ? r.w[e / 4][e % 4] : e % 2 ? r.w[0][e / 2] & 0xffff0000u : r.w[0][e / 2] << 16);
             if (infinite) x = x == INFINITY ? 0.f : -INFINITY;
             f(i + e, x);
         }
     }
-    template <typename F>
-    __device__ __forceinline__ void each(F&& f) const {
-        if constexpr (HELD) {
-#pragma unroll
-            for (int it = 0; it < HELD_ITS; ++it)
-                if (it < its) each8(it, f);
-        } else {
-            for (int it = 0; it < its; ++it) each8(it, f);
+    // g(it, raw) for each iteration that has tokens, the next one's on their way
+    template <typename G>
+    __device__ __forceinline__ void blocks(G&& g) const {
+        const int n = min(its, (V - start + BLOCK - 1) / BLOCK);
+        if (n <= 0) return;
+        Raw next = load8(0);
+        for (int it = 0; it < n; ++it) {
+            const Raw now = next;
+            if (it + 1 < n) next = load8(it + 1);
+            g(it, now);
         }
     }
-    // f(it, first index of the iteration)
     template <typename F>
-    __device__ __forceinline__ void blocks(F&& f) const {
-        if constexpr (HELD) {
+    __device__ __forceinline__ void each(F&& f) const {
+        blocks([&](int it, const Raw& r) { each8(it, r, f); });
+    }
+    // The first index at which the sums of measure(i, x), by index, reach
+    // want(sum of all), which is at least 1 and at most that.
+    template <typename W, typename M>
+    __device__ __forceinline__ int find(Shared& sh, W&& want_of, M&& measure) const {
+        clear(sh);
+        blocks([&](int it, const Raw& r) {
+            u64 s = 0;
+            each8(it, r, [&](int i, float x) { s += measure(i, x); });
+            s = wave_sum(s);
+            if (lane == 0) sh.hist[start / BLOCK + it] = s;
+        });
+        u64 want = locate(sh, want_of);
+        const int it = sh.bin - start / BLOCK;
+        if (it >= 0 && it < its) {
+            want -= sh.above;
+            const Raw r = load8(it);
+            u64 s[8];
+            int e = 0;
+            each8(it, r, [&](int i, float x) {
+                s[e] = measure(i, x) + (e ? s[e - 1] : 0);
+                ++e;
+            });
+            const u64 before = wave_scan(s[7]) - s[7];
+            if (before < want && before + s[7] >= want) {
+                int n = 0;
 #pragma unroll
-            for (int it = 0; it < HELD_ITS; ++it)
-                if (it < its) f(it);
-        } else {
-            for (int it = 0; it < its; ++it) f(it);
+                for (int j = 0; j < 7; ++j) n += before + s[j] < want;
+                sh.index = start + it * BLOCK + lane * 8 + n;
+            }
         }
+        __syncthreads();
+        return sh.index;
+    }
+    // Lists the tokens that `has` in index order, if they fit; their number.
+    template <typename H>
+    __device__ __forceinline__ int list(Shared& sh, H&& has) const {
+        int c = 0;
+        each([&](int i, float x) { c += has(i, x); });
+        c = __builtin_amdgcn_readlane(wave_scan(c), 63);
+        __syncthreads();
+        if (lane == 0) sh.ints[threadIdx.x / WAVE] = c;
+        __syncthreads();
+        int all, at = before_wave(sh.ints, &all);
+        if (all > NB || !c) {
+            __syncthreads();
+            return all;
+        }
+        blocks([&](int it, const Raw& r) {
+            int n = 0;
+            each8(it, r, [&](int i, float x) { n += has(i, x); });
+            const int run = wave_scan(n);
+            int to = at + run - n;
+            at += __builtin_amdgcn_readlane(run, 63);
+            if (n) each8(it, r, [&](int i, float x) {
+                if (has(i, x)) sh.list_x[to] = x, sh.list_i[to] = i, ++to;
+            });
+        });
+        __syncthreads();
+        return all;
     }
 };
 
-__device__ __forceinline__ void clear(Shared& sh) {
-    __syncthreads();
-    sh.hist[threadIdx.x] = sh.hist[threadIdx.x + THREADS] = 0;
-    __syncthreads();
-}
-
-__device__ __forceinline__ float2 range_of(Shared& sh, float lo, float hi) {
+// The tokens that a cut left: i is their place in the list, two a thread.
+struct List {
+    Shared* sh;
+    int n;
+    template <typename F>
+    __device__ __forceinline__ void each(F&& f) const {
 #pragma unroll
-    for (int o = 1; o < WAVE; o <<= 1) {
-        lo = fminf(lo, __shfl_xor(lo, o, WAVE));
-        hi = fmaxf(hi, __shfl_xor(hi, o, WAVE));
-    }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh.lo[threadIdx.x / WAVE] = lo, sh.hi[threadIdx.x / WAVE] = hi;
-    __syncthreads();
-    for (int w = 0; w < WAVES; ++w) lo = fminf(lo, sh.lo[w]), hi = fmaxf(hi, sh.hi[w]);
-    return make_float2(lo, hi);
-}
-
-// The first index at which the sums of measure(i, x), by index, reach `want`
-// (>= 1, at most all of them).
-template <typename R, typename M>
-__device__ __forceinline__ int find_by_index(Shared& sh, const R& row, u64 want, M&& measure) {
-    clear(sh);
-    row.blocks([&](int it) {
-        u64 s = 0;
-        row.each8(it, [&](int i, float x) { s += measure(i, x); });
-#pragma unroll
-        for (int o = 1; o < WAVE; o <<= 1) s += __shfl_xor(s, o, WAVE);
-        if (row.lane == 0) sh.hist[row.start / BLOCK + it] = s;
-    });
-    locate(sh, want);
-    const int block = sh.bin;
-    want -= sh.above;
-    row.blocks([&](int it) {
-        if (row.start / BLOCK + it != block) return;
-        u64 s = 0;
-        row.each8(it, [&](int i, float x) { s += measure(i, x); });
-        u64 run = wave_scan(s) - s;
-        if (run < want && run + s >= want) {
-            int found = 0x7fffffff;
-            row.each8(it, [&](int i, float x) {
-                const u64 w = measure(i, x);
-                if (run < want && run + w >= want) found = i;
-                run += w;
-            });
-            sh.index = found;
+        for (int e = 0; e < 2; ++e) {
+            const int i = 2 * threadIdx.x + e;
+            if (i < n) f(i, sh->list_x[i]);
         }
-    });
-    __syncthreads();
-    return sh.index;
-}
-
-// The shortest prefix of the order whose measure reaches `want` (>= 1): sh.hist
-// holds the first division of the measure, by step(x).  all: that is no prefix
-// but everything.  Tokens take part where measure(i, x) is not 0.
-template <typename R, typename M, typename Step>
-__device__ __forceinline__ Prefix shortest(Shared& sh, const R& row, u64 want, Prefix all, M&& measure, Step&& step) {
-    locate(sh, want);
-    if (sh.bin >= NB - 1) return all;  // the last step's tokens weigh nothing
-    int bin = sh.bin;
-    float lo = INFINITY, hi = -INFINITY;
-    row.each([&](int i, float x) {
-        if (step(x) == bin && all.has(x, i)) lo = fminf(lo, x), hi = fmaxf(hi, x);
-    });
-    want -= sh.above;
-    float2 r = range_of(sh, lo, hi);
-    while (r.x < r.y) {
-        // the ends fall into different steps, so this ends
-        const double top = (double)r.y, c = (NB - 1) / (top - (double)r.x);
-        auto finer = [&](float x) { return min(NB - 1, (int)((top - (double)x) * c)); };
-        clear(sh);
-        row.each([&](int i, float x) {
-            if (x >= r.x && x <= r.y) {
-                const u64 w = measure(i, x);
-                if (w) atomicAdd(&sh.hist[finer(x)], w);
-            }
-        });
-        locate(sh, want);
-        bin = sh.bin;
-        want -= sh.above;
-        lo = INFINITY, hi = -INFINITY;
-        row.each([&](int i, float x) {
-            if (x >= r.x && x <= r.y && finer(x) == bin && all.has(x, i)) lo = fminf(lo, x), hi = fmaxf(hi, x);
-        });
-        r = range_of(sh, lo, hi);
     }
-    const float x0 = r.x;
-    return {x0, find_by_index(sh, row, want, [&](int i, float x) { return x == x0 ? measure(i, x) : 0ull; })};
+    template <typename W, typename M>
+    __device__ __forceinline__ int find(Shared& s, W&& want_of, M&& measure) const {
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int i = 2 * threadIdx.x + e;
+            s.hist[i] = i < n ? measure(i, s.list_x[i]) : 0;
+        }
+        locate(s, want_of);
+        return s.bin;
+    }
+};
+
+// The shortest prefix of the order whose measure reaches want(the measure of all).
+// step(x) divides the logits into NB falling steps; the last one's tokens weigh
+// nothing.  Tokens with a measure of 0 take no part.  `all`, where the number is
+// never reached.
+template <typename T, typename W, typename M, typename Step>
+__device__ __forceinline__ Prefix shortest(Shared& sh, const T& tokens, Prefix all, W&& want_of, M&& measure, Step&& step) {
+    clear(sh);
+    tokens.each([&](int i, float x) {
+        const u64 w = measure(i, x);
+        if (w) atomicAdd(&sh.hist[step(x)], w);
+    });
+    u64 want = locate(sh, want_of);
+    if (sh.bin >= NB - 1) return all;
+    float top = 0.f, bottom = 0.f;  // of the last division, if `again`
+    double c = 0.;
+    bool again = false;
+    for (;;) {
+        const int bin = sh.bin;
+        want -= sh.above;
+        if (threadIdx.x == 0) sh.count = 0;
+        if (threadIdx.x < CAND) sh.cand_before[threadIdx.x] = 0;
+        __syncthreads();
+        float lo = INFINITY, hi = -INFINITY;
+        auto inside = [&](float x) {
+            return again ? x >= bottom && x <= top && min(NB - 1, (int)(((double)top - (double)x) * c)) == bin : step(x) == bin;
+        };
+        tokens.each([&](int i, float x) {
+            if (!inside(x)) return;
+            const u64 w = measure(i, x);
+            if (!w) return;
+            lo = fminf(lo, x), hi = fmaxf(hi, x);
+            const int at = atomicAdd(&sh.count, 1);
+            if (at < CAND) sh.cand_x[at] = x, sh.cand_i[at] = i, sh.cand_m[at] = w;
+        });
+        __syncthreads();
+        const int n = sh.count;
+        if (n <= CAND) {
+            // every eighth candidate before this thread's one, from its own first on
+            const int me = threadIdx.x & (CAND - 1), from = threadIdx.x / CAND;
+            const float x = sh.cand_x[me];
+            const int i = sh.cand_i[me];
+            if (me < n) {
+                u64 s = 0;
+                for (int j = from; j < n; j += THREADS / CAND) {
+                    const float y = sh.cand_x[j];
+                    if (y > x || (y == x && sh.cand_i[j] < i)) s += sh.cand_m[j];
+                }
+                if (s) atomicAdd(&sh.cand_before[me], s);
+            }
+            __syncthreads();
+            if (threadIdx.x < n) {
+                const u64 s = sh.cand_before[me];
+                if (s < want && s + sh.cand_m[me] >= want) sh.px = x, sh.pi = i;
+            }
+            __syncthreads();
+            return {sh.px, sh.pi};
+        }
+        const float2 r = block_range(sh, lo, hi);
+        if (r.x == r.y) {
+            const float x0 = r.x;
+            return {x0, tokens.find(sh, [&](u64) { return want; }, [&](int i, float x) { return x == x0 ? measure(i, x) : 0ull; })};
+        }
+        // the ends fall into different steps, so this ends
+        again = true;
+        bottom = r.x, top = r.y;
+        c = (NB - 1) / ((double)top - (double)bottom);
+        clear(sh);
+        tokens.each([&](int i, float x) {
+            if (!(x >= bottom && x <= top)) return;
+            const u64 w = measure(i, x);
+            if (w) atomicAdd(&sh.hist[min(NB - 1, (int)(((double)top - (double)x) * c))], w);
+        });
+        locate(sh, [&](u64) { return want; });
+    }
 }
 
-template <bool F32, bool HELD>
-__global__ void __launch_bounds__(THREADS) smg_sample_t(SampleArgs a) {
+__device__ __forceinline__ u64 share(float p, u64 all) {  // the measure that top-p asks for
+    const double want = ceil((double)p * (double)all);
+    return want >= 1. ? (u64)want : 1;
+}
+
+// The first token by index at which the weights that `kept` and min-p leave reach
+// more than u of their sum.
+template <typename T>
+__device__ __forceinline__ int draw(Shared& sh, const T& tokens, const Weigh& weigh, Prefix kept, float u, float min_p) {
+    const double least = min_p > 0.f ? fmin((double)min_p, 1.) * weigh.units : 0.;
+    return tokens.find(
+        sh,
+        [&](u64 all) {
+            const double aim = u > 0.f ? (double)u * (double)all : 0.;
+            return aim < (double)all ? (u64)aim + 1 : all;
+        },
+        [&](int i, float x) {
+            if (!kept.has(x, i) || (least > 0. && weigh.scaled(x) < least)) return 0ull;
+            return weigh.fixed(x);
+        });
+}
+
+template <bool F32>
+__global__ void __launch_bounds__(THREADS, 8) smg_sample_t(SampleArgs a) {
     __shared__ Shared sh;
     const int r = blockIdx.x, tid = threadIdx.x;
-    Row<F32, HELD> row;
+    Row<F32> row;
     row.init(a);
-    if (tid < 64) sh.pow2[tid] = exp2((double)tid / 64);
 
     float lo = INFINITY, hi = -INFINITY;
     row.each([&](int, float x) {
         hi = fmaxf(hi, x);  // NaN is passed over
         if (x > -INFINITY) lo = fminf(lo, x);
     });
-    float2 ends = range_of(sh, lo, hi);
+    float2 ends = block_range(sh, lo, hi);
     const float t = a.temperature[r];
     if (ends.y == -INFINITY) {
         if (tid == 0) a.out[r] = -1;
@@ -326,8 +471,8 @@ __global__ void __launch_bounds__(THREADS) smg_sample_t(SampleArgs a) {
     }
     if (!(t > 0.f)) {
         int first = 0x7fffffff;
-        row.each([&](int i, float x) { if (x == ends.y) first = min(first, i); });
         if (tid == 0) sh.index = 0x7fffffff;
+        row.each([&](int i, float x) { if (x == ends.y) first = min(first, i); });
         __syncthreads();
         if (first != 0x7fffffff) atomicMin(&sh.index, first);
         __syncthreads();
@@ -345,58 +490,37 @@ __global__ void __launch_bounds__(THREADS) smg_sample_t(SampleArgs a) {
     const float per = depth > 1e-30f ? (NB - 2) / depth : 0.f;
     auto step = [&](float x) { return (int)fminf((ends.y - x) * per, NB - 1.f); };
 
-    Prefix kept = {-INFINITY, -1};
+    Prefix kept = {-INFINITY, -1};  // everything above -inf
     const int k = a.top_k ? a.top_k[r] : 0;
-    const bool cut = k > 0 && k < a.V;
-    if (cut) {
-        clear(sh);
-        row.each([&](int, float x) {
-            if (x > -INFINITY) atomicAdd(&sh.hist[step(x)], 1ull);
-        });
-        kept = shortest(sh, row, (u64)k, kept, [](int, float x) { return (u64)(x > -INFINITY); }, step);
-    }
     const float p = a.top_p ? a.top_p[r] : 1.f;
-    if (p < 1.f) {
-        auto mass = [&](int i, float x) { return kept.has(x, i) ? weigh.fixed(x) : 0ull; };
-        clear(sh);
-        row.each([&](int i, float x) {
-            const u64 w = mass(i, x);
-            if (w) atomicAdd(&sh.hist[step(x)], w);
-        });
-        locate(sh, 1);
-        const double want = ceil((double)p * (double)sh.total);
-        const Prefix all = kept;
-        kept = shortest(sh, row, want >= 1. ? (u64)want : 1, all, mass, step);
-    }
     const float mp = a.min_p ? a.min_p[r] : 0.f;
-    const double least = mp > 0.f ? fmin((double)mp, 1.) : 0.;
-    auto last = [&](int i, float x) {
-        if (!kept.has(x, i)) return 0ull;
-        if (least > 0. && weigh.value(x) < least) return 0ull;
-        return weigh.fixed(x);
-    };
-    u64 s = 0;
-    row.each([&](int i, float x) { s += last(i, x); });
-#pragma unroll
-    for (int o = 1; o < WAVE; o <<= 1) s += __shfl_xor(s, o, WAVE);
-    __syncthreads();
-    if ((tid & 63) == 0) sh.part[tid / WAVE] = s;
-    __syncthreads();
-    u64 all = 0;
-    for (int w = 0; w < WAVES; ++w) all += sh.part[w];
     const float u = a.u[r];
-    const double aim = u > 0.f ? (double)u * (double)all : 0.;
-    const u64 want = aim < (double)all ? (u64)aim + 1 : all;  // the first sum above it
-    const int found = find_by_index(sh, row, want, last);
+    const Prefix all = kept;
+    auto live = [&](int i, float x) { return kept.has(x, i); };
+    List list = {&sh, NB + 1};
+    bool nucleus = p < 1.f;
+    if (k > 0 && k < a.V) {
+        kept = shortest(sh, row, all, [&](u64) { return (u64)k; }, [](int, float x) { return (u64)(x > -INFINITY); }, step);
+        list.n = row.list(sh, live);
+    }
+    if (nucleus && list.n > NB) {
+        kept = shortest(
+            sh, row, kept, [&](u64 sum) { return share(p, sum); },
+            [&](int i, float x) { return kept.has(x, i) ? weigh.fixed(x) : 0ull; }, step);
+        list.n = row.list(sh, live);
+        nucleus = false;
+    }
+    int found;
+    if (list.n <= NB) {
+        kept = all;
+        if (nucleus)
+            kept = shortest(
+                sh, list, all, [&](u64 sum) { return share(p, sum); }, [&](int, float x) { return weigh.fixed(x); }, step);
+        found = sh.list_i[draw(sh, list, weigh, kept, u, mp)];
+    } else {
+        found = draw(sh, row, weigh, kept, u, mp);
+    }
     if (tid == 0) a.out[r] = found;
-}
-
-template <bool F32>
-void launch(const SampleArgs& a, hipStream_t s) {
-    if (false)
-        hipLaunchKernelGGL((smg_sample_t<F32, true>), dim3(a.R), dim3(THREADS), 0, s, a);
-    else
-        hipLaunchKernelGGL((smg_sample_t<F32, false>), dim3(a.R), dim3(THREADS), 0, s, a);
 }
 
 }  // namespace
@@ -409,8 +533,8 @@ extern "C" int smg_sample_launch(const void* logits, const void* u, const void* 
     SampleArgs a = {logits, stride, (const float*)u, (const float*)temperature, (const int*)top_k,
                     (const float*)top_p, (const float*)min_p, (long long*)out, R, V};
     if (f32)
-        launch<true>(a, (hipStream_t)stream);
+        hipLaunchKernelGGL(smg_sample_t<true>, dim3(R), dim3(THREADS), 0, (hipStream_t)stream, a);
     else
-        launch<false>(a, (hipStream_t)stream);
+        hipLaunchKernelGGL(smg_sample_t<false>, dim3(R), dim3(THREADS), 0, (hipStream_t)stream, a);
     return hipGetLastError() == hipSuccess ? 0 : -2;
 }
