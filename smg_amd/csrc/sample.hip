@@ -165,7 +165,7 @@ __device__ __forceinline__ u64 locate(Shared& sh, W&& want_of) {
 struct Prefix {
     float x;
     int i;
-    __device__ __forceinline__ bool has(float y, int j) const { return y > x || (y == x && j <= i); }
+    __device__ __forceinline__ bool has(float y, int j) const { return (y > x) | ((y == x) & (j <= i)); }
 };
 
 // exp((x - top) / t) in 64 bits: 2^(n/64) from a table times a polynomial of
@@ -173,20 +173,22 @@ struct Prefix {
 struct Weigh {
     const double* pow2;
     double top, c, units;
-    float floor;  // below it weights are 0
+    float floor, cap;  // below the floor weights are 0; +inf weighs as the cap
     __device__ __forceinline__ void init(Shared& sh, float largest, float t, int V) {
         const int S = min(50, 62 - (V > 1 ? 32 - __clz(V - 1) : 0));
         units = (double)(1ull << S);
         pow2 = sh.pow2;
-        top = (double)largest;
+        // where the largest is +inf, only that weighs anything
+        cap = fminf(largest, 3.40282347e38f);
+        top = (double)cap;
         c = 64. * 1.44269504088896340736 / (double)t;
-        floor = fmaxf(largest - 45.f * t, -3.40282347e38f);  // 2^-64
+        floor = largest == INFINITY ? INFINITY : fmaxf(largest - 45.f * t, -3.40282347e38f);  // 2^-64
         if (threadIdx.x < 64) sh.pow2[threadIdx.x] = exp2((double)threadIdx.x / 64) * units;
     }
     __device__ __forceinline__ double scaled(float x) const {  // weight * 2^S
         constexpr double magic = 6755399441055744., q = 0.6931471805599453094 / 64;
-        const double d = (double)fmaxf(x, floor) - top;  // NaN and -inf too go to the floor
-        const double n = fma(d, c, magic);  // the nearest integer in its low bits
+        const double d = (double)fminf(fmaxf(x, floor), cap) - top;  // NaN goes to the floor
+        const double n = fma(d, c, magic);                           // the nearest integer in its low bits
         const double r = fma(d, c, magic - n);
         double p = fma(r, q * q * q * q / 24, q * q * q / 6);
         p = fma(r, p, q * q / 2);
@@ -197,37 +199,58 @@ struct Weigh {
         // times 2^(k/64): to the exponent, which stays in range (above 2^-66)
         return __longlong_as_double(bits + ((long long)(k & ~63) << 46));
     }
-    __device__ __forceinline__ u64 fixed(float x) const {
-        const u64 w = (u64)__double_as_longlong(scaled(x) + 4503599627370496.) & 0xfffffffffffffull;
-        return x >= floor ? w : 0;
+    __device__ __forceinline__ u64 rounded(double scaled) const {
+        return (u64)__double_as_longlong(scaled + 4503599627370496.) & 0xfffffffffffffull;
+    }
+    __device__ __forceinline__ u64 fixed(float x, bool live) const {
+        const u64 w = rounded(scaled(x));
+        return live & (x >= floor) ? w : 0;
     }
 };
 
 // ---- the tokens: f(i, x) for each of the thread's, in index order ---------------
-template <bool F32>
+// FEW: V < 8, where 8 tokens cannot be loaded at once.
+template <bool F32, bool FEW>
 struct Row {
     const char* at;
     int V, start, its, lane;
-    bool infinite;  // the largest is +inf: those weigh 1, all others nothing
 
     struct Raw {
         u32x4 w[F32 ? 2 : 1];
+        __device__ __forceinline__ float operator[](int e) const {
+            return __uint_as_float(F32 ? w[e / 4][e % 4] : e % 2 ? w[0][e / 2] & 0xffff0000u : w[0][e / 2] << 16);
+        }
+        __device__ __forceinline__ void drop(int e) {
+            if (F32)
+                w[e / 4][e % 4] = 0x7fc00000u;
+            else
+                w[0][e / 2] = e % 2 ? (w[0][e / 2] & 0xffffu) | 0x7fc00000u : (w[0][e / 2] & 0xffff0000u) | 0x7fc0u;
+        }
     };
+    // the first of an iteration's 8 tokens, and the first that is in memory: at the
+    // row's end a lane reads the last 8 and drops those before its own
+    __device__ __forceinline__ int first(int it) const { return start + it * BLOCK + lane * 8; }
+    __device__ __forceinline__ int base(int it) const { return FEW ? first(it) : min(first(it), V - 8); }
     __device__ __forceinline__ Raw load8(int it) const {
-        const int i = start + it * BLOCK + lane * 8;
-        Raw r;
-        if (i + 8 <= V) {
-            // rows may start anywhere: the hardware takes wide loads at any element
-            __builtin_memcpy(&r, at + (size_t)i * (F32 ? 4 : 2), F32 ? 32 : 16);
-        } else {
+        const int i = first(it), b = base(it);
+        Raw r = {};
+        if constexpr (FEW) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
+                r.drop(e);
+                if (i + e >= V) continue;
                 if (F32)
-                    r.w[e / 4][e % 4] = i + e < V ? ((const unsigned*)at)[i + e] : 0x7fc00000u;
-                else {
-                    const unsigned h = i + e < V ? ((const unsigned short*)at)[i + e] : 0x7fc0u;
-                    r.w[0][e / 2] = e % 2 ? r.w[0][e / 2] | h << 16 : h;
-                }
+                    r.w[e / 4][e % 4] = ((const unsigned*)at)[i + e];
+                else
+                    r.w[0][e / 2] = (r.w[0][e / 2] & (e % 2 ? 0xffffu : 0xffff0000u)) | (unsigned)((const unsigned short*)at)[i + e] << (e % 2 * 16);
+            }
+        } else {
+            // rows may start anywhere: the hardware takes wide loads at any element
+            __builtin_memcpy(&r, at + (size_t)b * (F32 ? 4 : 2), F32 ? 32 : 16);
+            if (b < i) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (b + e < i) r.drop(e);
             }
         }
         return r;
@@ -238,17 +261,12 @@ struct Row {
         at = (const char*)a.logits + blockIdx.x * a.stride * (F32 ? 4 : 2);
         its = (V + WAVES * BLOCK - 1) / (WAVES * BLOCK);
         start = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE) * its * BLOCK;
-        infinite = false;
     }
     template <typename F>
     __device__ __forceinline__ void each8(int it, const Raw& r, F&& f) const {
-        const int i = start + it * BLOCK + lane * 8;
+        const int b = base(it);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float x = __uint_as_float(F32 ? r.w[e / 4][e % 4] : e % 2 ? r.w[0][e / 2] & 0xffff0000u : r.w[0][e / 2] << 16);
-            if (infinite) x = x == INFINITY ? 0.f : -INFINITY;
-            f(i + e, x);
-        }
+        for (int e = 0; e < 8; ++e) f(b + e, r[e]);
     }
     // g(it, raw) for each iteration that has tokens, the next one's on their way
     template <typename G>
@@ -283,17 +301,14 @@ struct Row {
             want -= sh.above;
             const Raw r = load8(it);
             u64 s[8];
-            int e = 0;
-            each8(it, r, [&](int i, float x) {
-                s[e] = measure(i, x) + (e ? s[e - 1] : 0);
-                ++e;
-            });
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e] = measure(base(it) + e, r[e]) + (e ? s[e - 1] : 0);
             const u64 before = wave_scan(s[7]) - s[7];
             if (before < want && before + s[7] >= want) {
                 int n = 0;
 #pragma unroll
                 for (int j = 0; j < 7; ++j) n += before + s[j] < want;
-                sh.index = start + it * BLOCK + lane * 8 + n;
+                sh.index = base(it) + n;
             }
         }
         __syncthreads();
@@ -353,81 +368,106 @@ struct List {
     }
 };
 
-// The shortest prefix of the order whose measure reaches want(the measure of all).
-// step(x) divides the logits into NB falling steps; the last one's tokens weigh
-// nothing.  Tokens with a measure of 0 take no part.  `all`, where the number is
-// never reached.
-template <typename T, typename W, typename M, typename Step>
-__device__ __forceinline__ Prefix shortest(Shared& sh, const T& tokens, Prefix all, W&& want_of, M&& measure, Step&& step) {
-    clear(sh);
-    tokens.each([&](int i, float x) {
-        const u64 w = measure(i, x);
-        if (w) atomicAdd(&sh.hist[step(x)], w);
-    });
-    u64 want = locate(sh, want_of);
-    if (sh.bin >= NB - 1) return all;
-    float top = 0.f, bottom = 0.f;  // of the last division, if `again`
-    double c = 0.;
-    bool again = false;
-    for (;;) {
-        const int bin = sh.bin;
-        want -= sh.above;
-        if (threadIdx.x == 0) sh.count = 0;
-        if (threadIdx.x < CAND) sh.cand_before[threadIdx.x] = 0;
-        __syncthreads();
-        float lo = INFINITY, hi = -INFINITY;
-        auto inside = [&](float x) {
-            return again ? x >= bottom && x <= top && min(NB - 1, (int)(((double)top - (double)x) * c)) == bin : step(x) == bin;
-        };
-        tokens.each([&](int i, float x) {
-            if (!inside(x)) return;
-            const u64 w = measure(i, x);
-            if (!w) return;
-            lo = fminf(lo, x), hi = fmaxf(hi, x);
-            const int at = atomicAdd(&sh.count, 1);
-            if (at < CAND) sh.cand_x[at] = x, sh.cand_i[at] = i, sh.cand_m[at] = w;
-        });
-        __syncthreads();
-        const int n = sh.count;
-        if (n <= CAND) {
-            // every eighth candidate before this thread's one, from its own first on
-            const int me = threadIdx.x & (CAND - 1), from = threadIdx.x / CAND;
-            const float x = sh.cand_x[me];
-            const int i = sh.cand_i[me];
-            if (me < n) {
-                u64 s = 0;
-                for (int j = from; j < n; j += THREADS / CAND) {
-                    const float y = sh.cand_x[j];
-                    if (y > x || (y == x && sh.cand_i[j] < i)) s += sh.cand_m[j];
-                }
-                if (s) atomicAdd(&sh.cand_before[me], s);
-            }
-            __syncthreads();
-            if (threadIdx.x < n) {
-                const u64 s = sh.cand_before[me];
-                if (s < want && s + sh.cand_m[me] >= want) sh.px = x, sh.pi = i;
-            }
-            __syncthreads();
-            return {sh.px, sh.pi};
-        }
-        const float2 r = block_range(sh, lo, hi);
-        if (r.x == r.y) {
-            const float x0 = r.x;
-            return {x0, tokens.find(sh, [&](u64) { return want; }, [&](int i, float x) { return x == x0 ? measure(i, x) : 0ull; })};
-        }
-        // the ends fall into different steps, so this ends
-        again = true;
-        bottom = r.x, top = r.y;
-        c = (NB - 1) / ((double)top - (double)bottom);
-        clear(sh);
-        tokens.each([&](int i, float x) {
-            if (!(x >= bottom && x <= top)) return;
-            const u64 w = measure(i, x);
-            if (w) atomicAdd(&sh.hist[min(NB - 1, (int)(((double)top - (double)x) * c))], w);
-        });
-        locate(sh, [&](u64) { return want; });
+// Finds the shortest prefix of the order whose measure reaches a number: counts, or
+// weights, of the tokens that `from` has.
+template <typename T, typename Step>
+struct Search {
+    Shared& sh;
+    const T& tokens;
+    const Weigh& weigh;
+    Step step;  // NB falling steps of the logit; the last one's tokens weigh nothing
+    bool counting;
+    Prefix from;
+
+    __device__ __forceinline__ u64 measure(int i, float x) const {
+        if (counting) return (u64)from.has(x, i);
+        return weigh.fixed(x, from.has(x, i));
     }
-}
+    // The step in which want(sum of all) is reached, NB - 1 or NB if it never is.
+    template <typename W>
+    __device__ __forceinline__ u64 divide(W&& want_of) const {
+        clear(sh);
+        if (counting)
+            tokens.each([&](int i, float x) {
+                if (from.has(x, i)) atomicAdd(&sh.hist[step(x)], 1ull);
+            });
+        else
+            tokens.each([&](int i, float x) {
+                const u64 w = weigh.fixed(x, from.has(x, i));
+                if (w) atomicAdd(&sh.hist[step(x)], w);
+            });
+        return locate(sh, want_of);
+    }
+    // The prefix, from the step `bin` in which `want` is reached and the measure
+    // `above` it.
+    __device__ __forceinline__ Prefix within(int bin, u64 above, u64 want) const {
+        float top = 0.f, bottom = 0.f;  // of the last division, if `again`
+        double c = 0.;
+        bool again = false;
+        for (;;) {
+            want -= above;
+            if (threadIdx.x == 0) sh.count = 0;
+            if (threadIdx.x < CAND) sh.cand_before[threadIdx.x] = 0;
+            __syncthreads();
+            float lo = INFINITY, hi = -INFINITY;
+            tokens.each([&](int i, float x) {
+                const bool inside = again ? x >= bottom && x <= top && min(NB - 1, (int)(((double)top - (double)x) * c)) == bin : step(x) == bin;
+                if (!inside) return;
+                const u64 w = measure(i, x);
+                if (!w) return;
+                lo = fminf(lo, x), hi = fmaxf(hi, x);
+                const int at = atomicAdd(&sh.count, 1);
+                if (at < CAND) sh.cand_x[at] = x, sh.cand_i[at] = i, sh.cand_m[at] = w;
+            });
+            __syncthreads();
+            const int n = sh.count;
+            if (n <= CAND) {
+                // every eighth candidate, from this thread's first on, that comes before
+                // this thread's own
+                const int me = threadIdx.x & (CAND - 1), first = threadIdx.x / CAND;
+                const float x = sh.cand_x[me];
+                const int i = sh.cand_i[me];
+                if (me < n) {
+                    u64 s = 0;
+                    for (int j = first; j < n; j += THREADS / CAND) {
+                        const float y = sh.cand_x[j];
+                        if (y > x || (y == x && sh.cand_i[j] < i)) s += sh.cand_m[j];
+                    }
+                    if (s) atomicAdd(&sh.cand_before[me], s);
+                }
+                __syncthreads();
+                if (threadIdx.x < n) {
+                    const u64 s = sh.cand_before[me];
+                    if (s < want && s + sh.cand_m[me] >= want) sh.px = x, sh.pi = i;
+                }
+                __syncthreads();
+                return {sh.px, sh.pi};
+            }
+            const float2 r = block_range(sh, lo, hi);
+            if (r.x == r.y) {
+                const float x0 = r.x;
+                return {x0, tokens.find(sh, [&](u64) { return want; }, [&](int i, float x) { return x == x0 ? measure(i, x) : 0ull; })};
+            }
+            // the ends fall into different steps, so this ends
+            again = true;
+            bottom = r.x, top = r.y;
+            c = (NB - 1) / ((double)top - (double)bottom);
+            clear(sh);
+            tokens.each([&](int i, float x) {
+                if (!(x >= bottom && x <= top)) return;
+                const u64 w = measure(i, x);
+                if (w) atomicAdd(&sh.hist[min(NB - 1, (int)(((double)top - (double)x) * c))], w);
+            });
+            locate(sh, [&](u64) { return want; });
+            bin = sh.bin, above = sh.above;
+        }
+    }
+    template <typename W>
+    __device__ __forceinline__ Prefix operator()(W&& want_of) const {
+        const u64 want = divide(want_of);
+        return sh.bin >= NB - 1 ? from : within(sh.bin, sh.above, want);
+    }
+};
 
 __device__ __forceinline__ u64 share(float p, u64 all) {  // the measure that top-p asks for
     const double want = ceil((double)p * (double)all);
@@ -436,7 +476,7 @@ __device__ __forceinline__ u64 share(float p, u64 all) {  // the measure that to
 
 // The first token by index at which the weights that `kept` and min-p leave reach
 // more than u of their sum.
-template <typename T>
+template <bool CUT, typename T>
 __device__ __forceinline__ int draw(Shared& sh, const T& tokens, const Weigh& weigh, Prefix kept, float u, float min_p) {
     const double least = min_p > 0.f ? fmin((double)min_p, 1.) * weigh.units : 0.;
     return tokens.find(
@@ -446,24 +486,25 @@ __device__ __forceinline__ int draw(Shared& sh, const T& tokens, const Weigh& we
             return aim < (double)all ? (u64)aim + 1 : all;
         },
         [&](int i, float x) {
-            if (!kept.has(x, i) || (least > 0. && weigh.scaled(x) < least)) return 0ull;
-            return weigh.fixed(x);
+            const double w = weigh.scaled(x);
+            const bool live = (x >= weigh.floor) & (w >= least);
+            return (CUT ? live & kept.has(x, i) : live) ? weigh.rounded(w) : 0ull;
         });
 }
 
-template <bool F32>
+template <bool F32, bool FEW>
 __global__ void __launch_bounds__(THREADS, 8) smg_sample_t(SampleArgs a) {
     __shared__ Shared sh;
     const int r = blockIdx.x, tid = threadIdx.x;
-    Row<F32> row;
+    Row<F32, FEW> row;
     row.init(a);
 
     float lo = INFINITY, hi = -INFINITY;
     row.each([&](int, float x) {
         hi = fmaxf(hi, x);  // NaN is passed over
-        if (x > -INFINITY) lo = fminf(lo, x);
+        lo = fminf(lo, x > -INFINITY ? x : lo);
     });
-    float2 ends = block_range(sh, lo, hi);
+    const float2 ends = block_range(sh, lo, hi);
     const float t = a.temperature[r];
     if (ends.y == -INFINITY) {
         if (tid == 0) a.out[r] = -1;
@@ -472,55 +513,91 @@ __global__ void __launch_bounds__(THREADS, 8) smg_sample_t(SampleArgs a) {
     if (!(t > 0.f)) {
         int first = 0x7fffffff;
         if (tid == 0) sh.index = 0x7fffffff;
-        row.each([&](int i, float x) { if (x == ends.y) first = min(first, i); });
+        row.each([&](int i, float x) { first = min(first, x == ends.y ? i : 0x7fffffff); });
         __syncthreads();
         if (first != 0x7fffffff) atomicMin(&sh.index, first);
         __syncthreads();
         if (tid == 0) a.out[r] = sh.index;
         return;
     }
-    row.infinite = ends.y == INFINITY;
-    if (row.infinite) ends = make_float2(0.f, 0.f);
     Weigh weigh;
     weigh.init(sh, ends.y, t, a.V);
 
     // steps down from the largest: to the smallest, or to where weights are 0
     // (below 2^-51), whose tokens the last step takes
-    const float depth = fminf(ends.y - ends.x, 51.f * 0.69314718f * t);
+    const float cap = weigh.cap;
+    const float depth = fminf(cap - ends.x, 51.f * 0.69314718f * t);
     const float per = depth > 1e-30f ? (NB - 2) / depth : 0.f;
-    auto step = [&](float x) { return (int)fminf((ends.y - x) * per, NB - 1.f); };
+    auto step = [&](float x) { return (int)fminf((cap - fminf(x, cap)) * per, NB - 1.f); };
 
-    Prefix kept = {-INFINITY, -1};  // everything above -inf
+    // everything above -inf, or the +inf
+    const Prefix all = {ends.y == INFINITY ? cap : -INFINITY, -1};
+    Prefix kept = all;
     const int k = a.top_k ? a.top_k[r] : 0;
     const float p = a.top_p ? a.top_p[r] : 1.f;
     const float mp = a.min_p ? a.min_p[r] : 0.f;
     const float u = a.u[r];
-    const Prefix all = kept;
-    auto live = [&](int i, float x) { return kept.has(x, i); };
+    const bool by_count = k > 0 && k < a.V, by_mass = p < 1.f;
     List list = {&sh, NB + 1};
-    bool nucleus = p < 1.f;
-    if (k > 0 && k < a.V) {
-        kept = shortest(sh, row, all, [&](u64) { return (u64)k; }, [](int, float x) { return (u64)(x > -INFINITY); }, step);
-        list.n = row.list(sh, live);
+    if (by_count) {
+        Search<Row<F32, FEW>, decltype(step)> search = {sh, row, weigh, step, true, all};
+        if (k <= THREADS / 2) {
+            // the threads' largest tokens alone bound the k-th of all: what lies in
+            // their k-th's step or above is few
+            clear(sh);
+            if (hi > all.x) atomicAdd(&sh.hist[step(hi)], 1ull);
+            locate(sh, [&](u64) { return (u64)k; });
+            const int bin = sh.bin;
+            if (bin < NB - 1) list.n = row.list(sh, [&](int i, float x) { return (step(x) <= bin) & all.has(x, i); });
+        }
+        if (list.n > NB) {
+            kept = search([&](u64) { return (u64)k; });
+            list.n = row.list(sh, [&](int i, float x) { return kept.has(x, i); });
+            if (list.n <= NB) kept = all;
+        } else {
+            Search<List, decltype(step)> among = {sh, list, weigh, step, true, all};
+            kept = among([&](u64) { return (u64)k; });
+        }
     }
-    if (nucleus && list.n > NB) {
-        kept = shortest(
-            sh, row, kept, [&](u64 sum) { return share(p, sum); },
-            [&](int i, float x) { return kept.has(x, i) ? weigh.fixed(x) : 0ull; }, step);
-        list.n = row.list(sh, live);
-        nucleus = false;
+    if (by_mass) {
+        auto want_of = [&](u64 sum) { return share(p, sum); };
+        if (list.n > NB) {
+            Search<Row<F32, FEW>, decltype(step)> search = {sh, row, weigh, step, false, kept};
+            const u64 want = search.divide(want_of);
+            const int bin = sh.bin;
+            const u64 above = sh.above;
+            if (bin < NB - 1) {
+                list.n = row.list(sh, [&](int i, float x) { return (step(x) <= bin) & kept.has(x, i); });
+                if (list.n <= NB) {
+                    Search<List, decltype(step)> among = {sh, list, weigh, step, false, all};
+                    kept = among.within(bin, above, want);
+                } else {
+                    kept = search.within(bin, above, want);
+                    list.n = NB + 1;
+                }
+            }
+        } else {
+            Search<List, decltype(step)> among = {sh, list, weigh, step, false, kept};
+            kept = among(want_of);
+        }
     }
     int found;
     if (list.n <= NB) {
-        kept = all;
-        if (nucleus)
-            kept = shortest(
-                sh, list, all, [&](u64 sum) { return share(p, sum); }, [&](int, float x) { return weigh.fixed(x); }, step);
-        found = sh.list_i[draw(sh, list, weigh, kept, u, mp)];
+        found = sh.list_i[draw<true>(sh, list, weigh, kept, u, mp)];
+    } else if (by_count || by_mass) {
+        found = draw<true>(sh, row, weigh, kept, u, mp);
     } else {
-        found = draw(sh, row, weigh, kept, u, mp);
+        found = draw<false>(sh, row, weigh, kept, u, mp);
     }
     if (tid == 0) a.out[r] = found;
+}
+
+template <bool F32>
+void launch(const SampleArgs& a, hipStream_t s) {
+    if (a.V < 8)
+        hipLaunchKernelGGL((smg_sample_t<F32, true>), dim3(a.R), dim3(THREADS), 0, s, a);
+    else
+        hipLaunchKernelGGL((smg_sample_t<F32, false>), dim3(a.R), dim3(THREADS), 0, s, a);
 }
 
 }  // namespace
@@ -533,8 +610,8 @@ extern "C" int smg_sample_launch(const void* logits, const void* u, const void* 
     SampleArgs a = {logits, stride, (const float*)u, (const float*)temperature, (const int*)top_k,
                     (const float*)top_p, (const float*)min_p, (long long*)out, R, V};
     if (f32)
-        hipLaunchKernelGGL(smg_sample_t<true>, dim3(R), dim3(THREADS), 0, (hipStream_t)stream, a);
+        launch<true>(a, (hipStream_t)stream);
     else
-        hipLaunchKernelGGL(smg_sample_t<false>, dim3(R), dim3(THREADS), 0, (hipStream_t)stream, a);
+        launch<false>(a, (hipStream_t)stream);
     return hipGetLastError() == hipSuccess ? 0 : -2;
 }
