@@ -19,98 +19,123 @@ from typing import Optional, Tuple
 
 import torch
 
-_CACHE_TYPES = (torch.bfloat16, torch.float8_e4m3fn)
+_BF16, _FP8, _I32, _I64, _F32 = (torch.bfloat16, torch.float8_e4m3fn, torch.int32, torch.int64, torch.float32)
+_CACHE_TYPES = (_BF16, _FP8)
 HEAD_DIMS = (64, 128)
 MAX_NODES = 64
 MAX_VOCAB = 1 << 20
 
+try:
+    from .. import _core
+except ImportError:  # refusals work without the built core; _launch says that it is missing
+    _core = None
 
-def _core():
-    from .. import _core as core
 
-    return core
-
-
-def _check(name: str, t: torch.Tensor, dtypes, dim: int, device=None) -> None:
+# The checks are written for speed: one condition a tensor, and the reasons only
+# where it fails.
+def _check(name: str, t, dtypes: tuple, dim: int, dev: Optional[int]) -> None:
+    if isinstance(t, torch.Tensor) and t.dtype in dtypes and t.dim() == dim and (dev is None or t.get_device() == dev):
+        return
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
     if t.dtype not in dtypes:
         raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
     if t.dim() != dim:
         raise ValueError(f"{name} must have {dim} dimensions, got {tuple(t.shape)}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    raise ValueError(f"{name} is on {t.device}, the other tensors are not")
 
 
-def _check_rows(name: str, t: torch.Tensor) -> None:
-    """The last dimension dense, and every row at a multiple of 16 bytes (8 in an 8-bit cache)."""
+def _rows(name: str, t: torch.Tensor) -> tuple:
+    """The strides but the last, of a tensor that is dense in its last dimension and
+    whose rows start at multiples of 16 bytes (8 in an 8-bit cache)."""
+    strides = t.stride()
     e = t.element_size()
     unit = 16 if e > 1 else 8
-    if t.numel() == 0:
-        return
-    if t.stride(-1) != 1:
-        raise ValueError(f"{name} must be dense in its last dimension, strides {t.stride()}")
-    if t.data_ptr() % unit or any(s * e % unit for s, n in zip(t.stride()[:-1], t.shape) if n > 1):
-        raise ValueError(f"{name}: rows must start at multiples of {unit} bytes, strides {t.stride()}")
+    at = t.data_ptr()
+    for s in strides[:-1]:
+        at |= s * e
+    if (strides[-1] != 1 or at % unit) and t.numel():
+        if strides[-1] != 1:
+            raise ValueError(f"{name} must be dense in its last dimension, strides {strides}")
+        if t.data_ptr() % unit or any(s * e % unit for s, n in zip(strides[:-1], t.shape) if n > 1):
+            raise ValueError(f"{name}: rows must start at multiples of {unit} bytes, strides {strides}")
+    return strides[:-1]
 
 
-def _check_index(name: str, t: torch.Tensor, shape: tuple, device, dtype=torch.int32) -> None:
-    _check(name, t, (dtype,), len(shape), device)
-    if tuple(t.shape) != shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous {shape}, got {tuple(t.shape)} with strides {t.stride()}")
+def _index(name: str, t, shape: tuple, dev: int, dtype: torch.dtype = _I32) -> int:
+    """The address of a contiguous tensor of that shape."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == dev and t.is_contiguous():
+        return t.data_ptr()
+    _check(name, t, (dtype,), len(shape), dev)
+    raise ValueError(f"{name} must be contiguous {shape}, got {tuple(t.shape)} with strides {t.stride()}")
 
 
-def _check_gpu(name: str, t: torch.Tensor) -> None:
-    if t.device.type != "cuda":
-        raise RuntimeError(f"{name} is on {t.device}: the operators run on a CUDA/HIP device")
-
-
-def _check_cache(k: torch.Tensor, v: torch.Tensor, q: torch.Tensor, H: int, D: int) -> Tuple[int, int, int]:
-    for name, t in (("k_cache", k), ("v_cache", v)):
-        _check(name, t, _CACHE_TYPES, 4, q.device)
-        _check_rows(name, t)
-    if k.shape != v.shape or k.dtype != v.dtype:
-        raise ValueError(f"k_cache {tuple(k.shape)} {k.dtype} and v_cache {tuple(v.shape)} {v.dtype} differ")
-    S, KVH, T, d = k.shape
+def _cache(k: torch.Tensor, v: torch.Tensor, dev: int, H: int, D: int) -> tuple:
+    """(slots, kv heads, positions) and the strides of both."""
+    _check("k_cache", k, _CACHE_TYPES, 4, dev)
+    _check("v_cache", v, _CACHE_TYPES, 4, dev)
+    shape = k.shape
+    if shape != v.shape or k.dtype is not v.dtype:
+        raise ValueError(f"k_cache {tuple(shape)} {k.dtype} and v_cache {tuple(v.shape)} {v.dtype} differ")
+    S, KVH, T, d = shape
     if d != D or D not in HEAD_DIMS:
         raise ValueError(f"head dim must be one of {HEAD_DIMS} and equal, got {D} over a cache of {d}")
-    if min(S, KVH, T) < 1 or H % KVH:
-        raise ValueError(f"{H} heads over a cache of {tuple(k.shape)}")
-    return S, KVH, T
+    if min(S, KVH, T) < 1 or H < 1 or H % KVH:
+        raise ValueError(f"{H} heads over a cache of {tuple(shape)}")
+    return S, KVH, T, _rows("k_cache", k) + _rows("v_cache", v)
 
 
 def _scale(scale: Optional[float], D: int) -> float:
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if scale is None:
+        return D ** -0.5
+    scale = float(scale)
     if not (scale > 0 and math.isfinite(scale)):
         raise ValueError(f"scale must be positive and finite, got {scale}")
     return scale
 
 
-def _out_like(out: Optional[torch.Tensor], q: torch.Tensor) -> torch.Tensor:
+def _out(out: Optional[torch.Tensor], q: torch.Tensor, dev: int) -> torch.Tensor:
     if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _check("out", out, (torch.bfloat16,), q.dim(), q.device)
+        return q.new_empty(q.shape)
+    _check("out", out, (_BF16,), q.dim(), dev)
     if out.shape != q.shape:
         raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
-    _check_rows("out", out)
     return out
 
 
-def _plan(rows: int, tiles_of, ctx: int, KVH: int, D: int) -> Tuple[int, int]:
-    """(waves along the query rows, splits of the keys) for sequences of about
-    `rows` rows a kv head and up to `ctx` keys; tiles_of(rows a tile) counts tiles."""
+def _on_gpu(name: str, t: torch.Tensor, dev: int) -> None:
+    if dev < 0:
+        raise RuntimeError(f"{name} is on {t.device}: the operators run on a CUDA/HIP device")
+    if _core is None:
+        raise RuntimeError("smg_amd._core (gfx950 kernels) is not built: run `python -m smg_amd.csrc.build`")
+
+
+def _launch(kernel, dev: int, *args) -> None:
+    """kernel(*args, stream), on the device's current stream and with that device current."""
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    if torch._C._cuda_getDevice() == dev:
+        kernel(*args, stream)
+    else:
+        with torch.cuda.device(dev):
+            kernel(*args, stream)
+
+
+def _plan(rows: int, seqs: int, total: int, ctx: int, KVH: int, D: int) -> Tuple[int, int]:
+    """(waves along the query rows, splits of the keys) for `seqs` sequences of about
+    `rows` rows a kv head, `total` in all, and up to `ctx` keys."""
     wr = 1 if rows <= 32 and D == 128 else 2 if rows <= 64 else 4
-    work = tiles_of(32 * wr) * KVH
+    work = (total // (32 * wr) + seqs) * KVH
     split = 1
-    while split < 64 and work * split < 512 and ctx // (split * 2) >= 256:
+    while split < 64 and work * split < 512 and ctx >= split * 512:
         split *= 2
     return wr, split
 
 
-def _parts(split: int, rows: int, D: int, device):
+def _parts(split: int, rows: int, D: int, q: torch.Tensor) -> tuple:
+    """Workspace of the splits' partial results: the tensor, and the addresses of its halves."""
     if split == 1:
         return None, 0, 0
-    part = torch.empty(split * rows * (D + 2), dtype=torch.float32, device=device)
+    part = torch.empty(split * rows * (D + 2), dtype=_F32, device=q.device)
     return part, part.data_ptr(), part.data_ptr() + split * rows * D * 4
 
 
@@ -130,31 +155,28 @@ def attn_prefill(
     long caches over the card (default: the cache's length).  Returns out
     [N, H, D]; rows that no sequence covers are not written.  A sequence whose slot
     lies outside the cache gets zeros."""
-    _check("q", q, (torch.bfloat16,), 3)
+    _check("q", q, (_BF16,), 3, None)
+    dev = q.get_device()
     N, H, D = q.shape
-    S, KVH, T = _check_cache(k_cache, v_cache, q, H, D)
-    _check_rows("q", q)
+    S, KVH, T, cache_strides = _cache(k_cache, v_cache, dev, H, D)
     B = slots.shape[0] if isinstance(slots, torch.Tensor) and slots.dim() else 0
-    _check_index("slots", slots, (B,), q.device)
-    _check_index("starts", starts, (B,), q.device)
-    _check_index("cu_seqlens", cu_seqlens, (B + 1,), q.device)
+    p_slots = _index("slots", slots, (B,), dev)
+    p_starts = _index("starts", starts, (B,), dev)
+    p_cu = _index("cu_seqlens", cu_seqlens, (B + 1,), dev)
     scale = _scale(scale, D)
-    out = _out_like(out, q)
-    _check_gpu("q", q)
+    out = _out(out, q, dev)
+    strides = _rows("q", q) + _rows("out", out) + cache_strides
+    _on_gpu("q", q, dev)
     if N == 0 or B == 0:
         return out
-    G = H // KVH
+    total = N * (H // KVH)
     ctx = T if max_ctx is None else max(1, min(int(max_ctx), T))
-    wr, split = _plan(N * G // B, lambda bm: N * G // bm + B, ctx, KVH, D)
-    with torch.cuda.device(q.device):
-        part, po, pm = _parts(split, N * H, D, q.device)
-        _core().attn_prefill(
-            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(), starts.data_ptr(),
-            cu_seqlens.data_ptr(), out.data_ptr(), po, pm,
-            [*q.stride()[:2], *out.stride()[:2], *k_cache.stride()[:3], *v_cache.stride()[:3]],
-            B, N, H, KVH, S, T, D, split, wr, scale, int(k_cache.dtype == torch.float8_e4m3fn),
-            torch.cuda.current_stream().cuda_stream,
-        )
+    wr, split = _plan(total // B, B, total, ctx, KVH, D)
+    part, po, pm = _parts(split, N * H, D, q)
+    _launch(
+        _core.attn_prefill, dev, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), p_slots, p_starts, p_cu,
+        out.data_ptr(), po, pm, strides, B, N, H, KVH, S, T, D, split, wr, scale, k_cache.dtype is _FP8,
+    )
     return out
 
 
@@ -174,38 +196,34 @@ def attn_tree(
 
     max_ctx, a bound on ctx_lens, only sizes the split of long caches over the
     card (default: the cache's length)."""
-    _check("q", q, (torch.bfloat16,), 4)
+    _check("q", q, (_BF16,), 4, None)
+    dev = q.get_device()
     B, N, H, D = q.shape
-    S, KVH, T = _check_cache(k_cache, v_cache, q, H, D)
-    _check_rows("q", q)
-    for name, t in (("k_new", k_new), ("v_new", v_new)):
-        _check(name, t, (torch.bfloat16,), 4, q.device)
-        if tuple(t.shape) != (B, N, KVH, D):
-            raise ValueError(f"{name} must be {(B, N, KVH, D)}, got {tuple(t.shape)}")
-        _check_rows(name, t)
+    S, KVH, T, cache_strides = _cache(k_cache, v_cache, dev, H, D)
+    _check("k_new", k_new, (_BF16,), 4, dev)
+    _check("v_new", v_new, (_BF16,), 4, dev)
+    if not k_new.shape == v_new.shape == (B, N, KVH, D):
+        raise ValueError(f"k_new and v_new must be {(B, N, KVH, D)}, got {tuple(k_new.shape)} and {tuple(v_new.shape)}")
     if N > MAX_NODES:
         raise ValueError(f"at most {MAX_NODES} drafted nodes, got {N}")
-    _check_index("slots", slots, (B,), q.device)
-    _check_index("ctx_lens", ctx_lens, (B,), q.device)
-    _check_index("parents", parents, (B, N), q.device)
+    p_slots = _index("slots", slots, (B,), dev)
+    p_ctx = _index("ctx_lens", ctx_lens, (B,), dev)
+    p_parents = _index("parents", parents, (B, N), dev)
     scale = _scale(scale, D)
-    out = _out_like(out, q)
-    _check_gpu("q", q)
+    out = _out(out, q, dev)
+    strides = _rows("q", q) + _rows("out", out) + cache_strides + _rows("k_new", k_new) + _rows("v_new", v_new)
+    _on_gpu("q", q, dev)
     if B == 0 or N == 0:
         return out
-    G = H // KVH
+    rows = N * (H // KVH)
     ctx = T if max_ctx is None else max(1, min(int(max_ctx), T))
-    wr, split = _plan(N * G, lambda bm: B * -(-N * G // bm), ctx, KVH, D)
-    with torch.cuda.device(q.device):
-        part, po, pm = _parts(split, B * N * H, D, q.device)
-        _core().attn_tree(
-            q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-            slots.data_ptr(), ctx_lens.data_ptr(), parents.data_ptr(), out.data_ptr(), po, pm,
-            [*q.stride()[:3], *out.stride()[:3], *k_cache.stride()[:3], *v_cache.stride()[:3],
-             *k_new.stride()[:3], *v_new.stride()[:3]],
-            B, N, H, KVH, S, T, D, split, wr, scale, int(k_cache.dtype == torch.float8_e4m3fn),
-            torch.cuda.current_stream().cuda_stream,
-        )
+    wr, split = _plan(rows, B, B * rows, ctx, KVH, D)
+    part, po, pm = _parts(split, B * N * H, D, q)
+    _launch(
+        _core.attn_tree, dev, q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+        p_slots, p_ctx, p_parents, out.data_ptr(), po, pm, strides, B, N, H, KVH, S, T, D, split, wr, scale,
+        k_cache.dtype is _FP8,
+    )
     return out
 
 
@@ -228,36 +246,29 @@ def tree_commit(
     sequence's next token.  A sequence whose slot lies outside the cache, that has
     no room or whose node 0 has a parent is padding: 0, -1, -1.  Of sequences that
     name the same slot the last one's rows are written."""
-    _check("kv_new", kv_new, (torch.bfloat16,), 6)
+    _check("kv_new", kv_new, (_BF16,), 6, None)
+    dev = kv_new.get_device()
     L, two, B, N, KVH, D = kv_new.shape
-    _check("kv_cache", kv_cache, _CACHE_TYPES, 6, kv_new.device)
+    _check("kv_cache", kv_cache, _CACHE_TYPES, 6, dev)
     S, T = kv_cache.shape[2], kv_cache.shape[4]
-    if two != 2 or tuple(kv_cache.shape) != (L, 2, S, KVH, T, D) or min(L, S, KVH, T, D) < 1:
+    if two != 2 or kv_cache.shape != (L, 2, S, KVH, T, D) or min(L, S, KVH, T, D) < 1:
         raise ValueError(f"kv_new {tuple(kv_new.shape)} does not fit kv_cache {tuple(kv_cache.shape)}")
     if D % 8:
         raise ValueError(f"head dim must be a multiple of 8, got {D}")
-    _check_rows("kv_new", kv_new)
-    _check_rows("kv_cache", kv_cache)
     if N > MAX_NODES or (N < 1 and B > 0):
         raise ValueError(f"1 to {MAX_NODES} drafted nodes, got {N}")
-    _check_index("slots", slots, (B,), kv_new.device)
-    _check_index("ctx_lens", ctx_lens, (B,), kv_new.device)
-    _check_index("parents", parents, (B, N), kv_new.device)
-    _check_index("tokens", tokens, (B, N), kv_new.device, torch.int64)
-    _check_index("targets", targets, (B, N), kv_new.device, torch.int64)
-    _check_gpu("kv_new", kv_new)
-    count = torch.empty(B, dtype=torch.int32, device=kv_new.device)
-    path = torch.empty(B, N, dtype=torch.int32, device=kv_new.device)
-    nxt = torch.empty(B, dtype=torch.int64, device=kv_new.device)
-    if B == 0:
-        return count, path, nxt
-    with torch.cuda.device(kv_new.device):
-        _core().tree_commit(
-            kv_new.data_ptr(), kv_cache.data_ptr(), slots.data_ptr(), ctx_lens.data_ptr(),
-            parents.data_ptr(), tokens.data_ptr(), targets.data_ptr(), count.data_ptr(),
-            path.data_ptr(), nxt.data_ptr(), [*kv_new.stride()[:5], *kv_cache.stride()[:5]],
-            B, N, L, KVH, S, T, D, int(kv_cache.dtype == torch.float8_e4m3fn),
-            torch.cuda.current_stream().cuda_stream,
+    strides = _rows("kv_new", kv_new) + _rows("kv_cache", kv_cache)
+    given = (
+        _index("slots", slots, (B,), dev), _index("ctx_lens", ctx_lens, (B,), dev),
+        _index("parents", parents, (B, N), dev), _index("tokens", tokens, (B, N), dev, _I64),
+        _index("targets", targets, (B, N), dev, _I64),
+    )
+    _on_gpu("kv_new", kv_new, dev)
+    count, path, nxt = ctx_lens.new_empty(B), parents.new_empty((B, N)), tokens.new_empty(B)
+    if B:
+        _launch(
+            _core.tree_commit, dev, kv_new.data_ptr(), kv_cache.data_ptr(), *given, count.data_ptr(), path.data_ptr(),
+            nxt.data_ptr(), strides, B, N, L, KVH, S, T, D, kv_cache.dtype is _FP8,
         )
     return count, path, nxt
 
@@ -281,30 +292,28 @@ def sample(
     and a token below half of that is never taken.  temperature (float32 [R]) 0
     takes the first token of the order.  -inf and NaN logits are never taken; a
     row of nothing else gives -1."""
-    _check("logits", logits, (torch.bfloat16, torch.float32), 2)
+    _check("logits", logits, (_BF16, _F32), 2, None)
+    dev = logits.get_device()
     R, V = logits.shape
     if not 1 <= V <= MAX_VOCAB:
         raise ValueError(f"1 to {MAX_VOCAB} columns of logits, got {V}")
-    if V > 1 and logits.stride(1) != 1:
+    stride, dense = logits.stride()
+    if V > 1 and dense != 1:
         raise ValueError(f"logits must be dense in their last dimension, strides {logits.stride()}")
-    dev = logits.device
-    _check_index("u", u, (R,), dev, torch.float32)
-    _check_index("temperature", temperature, (R,), dev, torch.float32)
-    for name, t, dtype in (("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
-        if t is not None:
-            _check_index(name, t, (R,), dev, dtype)
+    rows = (R,)
+    p_u = _index("u", u, rows, dev, _F32)
+    p_temperature = _index("temperature", temperature, rows, dev, _F32)
+    p_k = 0 if top_k is None else _index("top_k", top_k, rows, dev)
+    p_p = 0 if top_p is None else _index("top_p", top_p, rows, dev, _F32)
+    p_m = 0 if min_p is None else _index("min_p", min_p, rows, dev, _F32)
     if out is not None:
-        _check_index("out", out, (R,), dev, torch.int64)
-    _check_gpu("logits", logits)
+        _index("out", out, rows, dev, _I64)
+    _on_gpu("logits", logits, dev)
     if out is None:
-        out = torch.empty(R, dtype=torch.int64, device=dev)
-    if R == 0:
-        return out
-    with torch.cuda.device(dev):
-        _core().sample(
-            logits.data_ptr(), u.data_ptr(), temperature.data_ptr(),
-            0 if top_k is None else top_k.data_ptr(), 0 if top_p is None else top_p.data_ptr(),
-            0 if min_p is None else min_p.data_ptr(), out.data_ptr(), logits.stride(0), R, V,
-            int(logits.dtype == torch.float32), torch.cuda.current_stream().cuda_stream,
+        out = torch.empty(rows, dtype=_I64, device=logits.device)
+    if R:
+        _launch(
+            _core.sample, dev, logits.data_ptr(), p_u, p_temperature, p_k, p_p, p_m, out.data_ptr(), stride, R, V,
+            logits.dtype is _F32,
         )
     return out
