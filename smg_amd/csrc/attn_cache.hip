@@ -114,24 +114,128 @@ __device__ __forceinline__ int k_chunk(int row, int c) {
     return row * (D / 8) + (c ^ (row & (D / 8 - 1)));
 }
 template <int D>
-__device__ __forceinline__ int v_chunk(int row, int c) {
-    const int x = D == 128 ? (row & 7) << 1 : ((row >> 1) & 3) << 1;
-    return row * (D / 8) + (c ^ x);
+__device__ __forceinline__ int v_swap(int row) {
+    return D == 128 ? (row & 7) << 1 : ((row >> 1) & 3) << 1;
 }
+template <int D>
+__device__ __forceinline__ int v_chunk(int row, int c) {
+    return row * (D / 8) + (c ^ v_swap<D>(row));
+}
+
+// 64 lanes' 16 bytes each straight to 1 KB of LDS at `to` (the same in all lanes)
+__device__ __forceinline__ void to_lds(const void* from, u32x4* to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                     (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+
+// a wave's scores, weights and sums over one tile
+template <int D, int KB>
+struct Tile {
+    static constexpr int HB = D / 32;
+    f32x16 acc[HB];  // O^T, unnormalised
+    float m, mc, l;  // the running maximum, m * c (0 where nothing is seen yet), the sum of this half
+
+    __device__ __forceinline__ void init() {
+#pragma unroll
+        for (int i = 0; i < HB; ++i) acc[i] = (f32x16)0.f;
+        m = -INFINITY;
+        mc = l = 0.f;
+    }
+    // keys w0 .. w0 + 32 KB - 1 of the tile; where MASKED, bit i of `seen` is key i of those
+    template <bool MASKED>
+    __device__ __forceinline__ void take(const u32x4* sk, const u32x4* sv, const bf16x8* qf, int w0, float c, unsigned long long seen) {
+        const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+        f32x16 s[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            s[kb] = (f32x16)0.f;
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) {
+                const bf16x8 kf = __builtin_bit_cast(bf16x8, sk[k_chunk<D>(w0 + kb * 32 + col, 2 * j + half)]);
+                s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[j], s[kb], 0, 0, 0);
+            }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if (MASKED && !((unsigned)(seen >> kb * 32) >> half * 4 & 1u << ((i >> 2) * 8 + (i & 3)))) s[kb][i] = -INFINITY;
+                top = fmaxf(top, s[kb][i]);
+            }
+        top = max_halves(top);
+        // the maximum follows only when a weight would pass 2^8: f32 and bf16 hold
+        // that as exactly, and the accumulators are seldom rescaled
+        if (__any((top - m) * c > 8.f)) {
+            const float m2 = fmaxf(m, top);
+            const float mc2 = m2 == -INFINITY ? 0.f : m2 * c;
+            const float alpha = __builtin_amdgcn_exp2f(m * c - mc2);
+            m = m2;
+            mc = mc2;
+            l *= alpha;
+#pragma unroll
+            for (int i = 0; i < HB; ++i) acc[i] *= alpha;
+        }
+        bf16x8 p[KB][2];
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(s[kb][i], c, -mc));
+                sum[i & 3] += e;
+                p[kb][i >> 3][i & 7] = (__bf16)e;
+            }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int hb = 0; hb < HB; ++hb) {
+                    // lane -> key rows r0 .. r0+3 (and r0+8 ..) of column hb*32 + col
+                    const int r0 = w0 + kb * 32 + j * 16 + half * 4 + ((lane & 15) >> 2);
+                    const int cc = hb * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+                    typedef __attribute__((address_space(3))) s16x4* lds_t;
+                    const char* lo = (const char*)&sv[v_chunk<D>(r0, cc)] + (lane & 1) * 8;
+                    const char* hi = (const char*)&sv[v_chunk<D>(r0 + 8, cc)] + (lane & 1) * 8;
+                    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)lo);
+                    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)hi);
+                    bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+                    if (MASKED) {
+                        // 0 * inf is NaN: a masked key's weight is 0, but its V must not
+                        // reach the rows that do not see it.  Such values are left out
+                        // here, and products of their own find the rows that they meet
+                        // with a weight.
+                        const u32x4 all = __builtin_bit_cast(u32x4, vf);
+                        u32x4 fin;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) fin[i] = all[i] & ~halves_where<BAD>(all[i]);
+                        vf = __builtin_bit_cast(bf16x8, fin);
+                        const u32x4 cut = fin ^ all;
+                        if (__any((cut[0] | cut[1] | cut[2] | cut[3]) != 0)) {
+                            add_where<PLUS>(acc[hb], all, p[kb][j], INFINITY);
+                            add_where<MINUS>(acc[hb], all, p[kb][j], -INFINITY);
+                            add_where<NOT>(acc[hb], all, p[kb][j], NAN);
+                        }
+                    }
+                    acc[hb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, p[kb][j], acc[hb], 0, 0, 0);
+                }
+    }
+};
 
 // TREE: drafted nodes with their own K/V after the context.  KV8: e4m3 cache.
 // WR waves share the query rows of a tile (32 each), WK = 4 / WR split its keys.
 template <bool TREE, bool KV8, int D, int WR>
-__global__ void __launch_bounds__(256, 2) smg_attn_cache_t(AttnArgs a) {
+__global__ void __launch_bounds__(256, WR == 4 ? 2 : 1) smg_attn_cache_t(AttnArgs a) {
     constexpr int WK = 4 / WR;
     constexpr int KB = WK == 4 ? 1 : 2;      // blocks of 32 keys a wave takes of a tile
     constexpr int BN = 32 * KB * WK;         // keys of a tile
     constexpr int BM = 32 * WR;              // query rows of a workgroup
     constexpr int CPR = D / 8;               // 16-byte chunks a row
     constexpr int HB = D / 32;
+    constexpr int STAGE = 2 * BN * CPR;      // chunks of a tile, K then V; two tiles in turn
     extern __shared__ u32x4 smem[];
-    u32x4* sk = smem;
-    u32x4* sv = smem + BN * CPR;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wr = wave % WR, wk = wave / WR;
@@ -198,28 +302,21 @@ __global__ void __launch_bounds__(256, 2) smg_attn_cache_t(AttnArgs a) {
     int limit;                        // cache rows <= limit
     unsigned long long nodes = 0;     // drafted nodes that this row sees
     if constexpr (TREE) {
-        __shared__ int up[64];
-        __shared__ unsigned long long seen[64];
-        if (tid < a.N) up[tid] = a.parents[(size_t)b * a.N + tid];
-        __syncthreads();
-        if (tid < a.N) {
-            // a parent comes before its child, so the walk ends; anything else
-            // below -1 or not before it marks a node that is not in the tree
-            unsigned long long m = 0;
-            int i = tid;
-            while (i >= 0) {
-                m |= 1ull << i;
-                const int p = up[i];
-                if (p >= i || p < -1) {
-                    m = 0;
-                    break;
-                }
-                i = p;
-            }
-            seen[tid] = m;
+        // A lane a node: ancestors by doubling.  A parent comes before its child;
+        // anything else below -1 or not before it marks a node outside the tree,
+        // which -2 hands down.
+        unsigned long long m = 1ull << lane;
+        int up = lane < a.N ? a.parents[(size_t)b * a.N + lane] : -2;
+        if (up >= lane || up < -1) up = -2;
+#pragma unroll
+        for (int i = 0; i < 6; ++i) {
+            const int from = max(up, 0);
+            const unsigned long long m2 = __shfl(m, from, WAVE);
+            const int up2 = __shfl(up, from, WAVE);
+            if (up >= 0) m |= m2, up = up2;
         }
-        __syncthreads();
-        nodes = live && cached ? seen[token] : 0;
+        nodes = __shfl(up == -1 ? m : 0ull, token, WAVE);
+        if (!live || !cached) nodes = 0;
         limit = nodes ? ctx - 1 : -1;
     } else {
         limit = live && cached ? min(ctx + token, a.T - 1) : -1;
@@ -245,114 +342,76 @@ __global__ void __launch_bounds__(256, 2) smg_attn_cache_t(AttnArgs a) {
     for (int o = 1; o < 32; o <<= 1) least = min(least, __shfl_xor(least, o, WAVE));
     least = __builtin_amdgcn_readfirstlane(least);
 
-    f32x16 acc[HB];
-#pragma unroll
-    for (int i = 0; i < HB; ++i) acc[i] = (f32x16)0.f;
-    float m = -INFINITY, l = 0.f;
-
-    for (int t = t0; t < t1; ++t) {
+    // Tile t to LDS: 16-bit rows straight from memory, permuted by where each lane
+    // reads; an 8-bit cache's by way of registers (`put` widens them later).
+    constexpr int PER = BN * CPR / 256;  // chunks a thread
+    constexpr int RPI = 64 / CPR;        // rows of a wave's 1 KB
+    uint2 k8[KV8 ? PER : 1], v8[KV8 ? PER : 1];
+    auto get = [&](int t, u32x4* to) {
         const bool fresh = TREE && t >= ctx_tiles;
         const int n0 = fresh ? (t - ctx_tiles) * BN : t * BN;
         const int nlast = (fresh ? a.N : kend) - 1;  // rows past the end repeat the last
-        __syncthreads();
-        for (int i = tid; i < BN * CPR; i += 256) {
-            const int r = i / CPR, cc = i % CPR;
-            const long long src = min(n0 + r, nlast);
-            u32x4 kx, vx;
-            if (KV8 && !fresh) {
-                const uint2 k8 = *(const uint2*)(kbase + src * a.k_st + cc * 8);
-                const uint2 v8 = *(const uint2*)(vbase + src * a.v_st + cc * 8);
-                kx = {fp8x2_to_bf16x2(k8.x, false), fp8x2_to_bf16x2(k8.x, true),
-                      fp8x2_to_bf16x2(k8.y, false), fp8x2_to_bf16x2(k8.y, true)};
-                vx = {fp8x2_to_bf16x2(v8.x, false), fp8x2_to_bf16x2(v8.x, true),
-                      fp8x2_to_bf16x2(v8.y, false), fp8x2_to_bf16x2(v8.y, true)};
-            } else {
-                const __hip_bfloat16* kr = fresh ? knew + src * a.kn_st : (const __hip_bfloat16*)kbase + src * a.k_st;
-                const __hip_bfloat16* vr = fresh ? vnew + src * a.vn_st : (const __hip_bfloat16*)vbase + src * a.v_st;
-                kx = *(const u32x4*)(kr + cc * 8);
-                vx = *(const u32x4*)(vr + cc * 8);
+        if (KV8 && !fresh) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int at = i * 256 + tid;
+                const long long src = min(n0 + at / CPR, nlast);
+                k8[i] = *(const uint2*)(kbase + src * a.k_st + at % CPR * 8);
+                v8[i] = *(const uint2*)(vbase + src * a.v_st + at % CPR * 8);
             }
-            sk[k_chunk<D>(r, cc)] = kx;
-            sv[v_chunk<D>(r, cc)] = vx;
+        } else {
+            const __hip_bfloat16* kp = fresh ? knew : (const __hip_bfloat16*)kbase;
+            const __hip_bfloat16* vp = fresh ? vnew : (const __hip_bfloat16*)vbase;
+            const long long ks = fresh ? a.kn_st : a.k_st, vs = fresh ? a.vn_st : a.v_st;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int r0 = (i * 4 + wave) * RPI, r = r0 + lane / CPR, cc = lane % CPR;
+                const long long src = min(n0 + r, nlast);
+                to_lds(kp + src * ks + (cc ^ (r & (CPR - 1))) * 8, to + r0 * CPR);
+                to_lds(vp + src * vs + (cc ^ v_swap<D>(r)) * 8, to + BN * CPR + r0 * CPR);
+            }
         }
-        __syncthreads();
+    };
+    auto put = [&](int t, u32x4* to) {
+        if (!KV8 || (TREE && t >= ctx_tiles)) return;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int r = (i * 256 + tid) / CPR, cc = tid % CPR;
+            to[k_chunk<D>(r, cc)] = u32x4{fp8x2_to_bf16x2(k8[i].x, false), fp8x2_to_bf16x2(k8[i].x, true),
+                                          fp8x2_to_bf16x2(k8[i].y, false), fp8x2_to_bf16x2(k8[i].y, true)};
+            to[BN * CPR + v_chunk<D>(r, cc)] = u32x4{fp8x2_to_bf16x2(v8[i].x, false), fp8x2_to_bf16x2(v8[i].x, true),
+                                                     fp8x2_to_bf16x2(v8[i].y, false), fp8x2_to_bf16x2(v8[i].y, true)};
+        }
+    };
 
-        const int w0 = wk * KB * 32;  // this wave's keys of the tile
-        const bool masked = fresh || n0 + w0 + KB * 32 - 1 > least;  // the same in the whole wave
-        f32x16 s[KB];
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-            s[kb] = (f32x16)0.f;
-#pragma unroll
-            for (int j = 0; j < D / 16; ++j) {
-                const bf16x8 kf = __builtin_bit_cast(bf16x8, sk[k_chunk<D>(w0 + kb * 32 + col, 2 * j + half)]);
-                s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[j], s[kb], 0, 0, 0);
-            }
-        }
-        float top = -INFINITY;
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                if (masked) {
-                    const int key = n0 + w0 + kb * 32 + (i >> 2) * 8 + half * 4 + (i & 3);
-                    const bool sees = fresh ? (key < 64 && (nodes >> (key & 63) & 1)) : key <= limit;
-                    if (!sees) s[kb][i] = -INFINITY;
-                }
-                top = fmaxf(top, s[kb][i]);
-            }
-        top = max_halves(top);
-        const float m2 = fmaxf(m, top);
-        const float mc = m2 == -INFINITY ? 0.f : m2 * c;  // nothing seen yet: every p is 2^-inf
-        const float alpha = exp2f(m * c - mc);
-        m = m2;
-        l *= alpha;
-#pragma unroll
-        for (int i = 0; i < HB; ++i) acc[i] *= alpha;
-        bf16x8 p[KB][2];
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float e = exp2f(fmaf(s[kb][i], c, -mc));
-                l += e;
-                p[kb][i >> 3][i & 7] = (__bf16)e;
-            }
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int hb = 0; hb < HB; ++hb) {
-                    // lane -> key rows r0 .. r0+3 (and r0+8 ..) of column hb*32 + col
-                    const int r0 = w0 + kb * 32 + j * 16 + half * 4 + ((lane & 15) >> 2);
-                    const int cc = hb * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
-                    typedef __attribute__((address_space(3))) s16x4* lds_t;
-                    const char* lo = (const char*)&sv[v_chunk<D>(r0, cc)] + (lane & 1) * 8;
-                    const char* hi = (const char*)&sv[v_chunk<D>(r0 + 8, cc)] + (lane & 1) * 8;
-                    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)lo);
-                    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)hi);
-                    bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-                    if (masked) {
-                        // 0 * inf is NaN: a masked key's weight is 0, but its V must not
-                        // reach the rows that do not see it.  Such values are left out
-                        // here, and products of their own find the rows that they meet
-                        // with a weight.
-                        const u32x4 all = __builtin_bit_cast(u32x4, vf);
-                        u32x4 fin;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) fin[i] = all[i] & ~halves_where<BAD>(all[i]);
-                        vf = __builtin_bit_cast(bf16x8, fin);
-                        const u32x4 cut = fin ^ all;
-                        if (__any((cut[0] | cut[1] | cut[2] | cut[3]) != 0)) {
-                            add_where<PLUS>(acc[hb], all, p[kb][j], INFINITY);
-                            add_where<MINUS>(acc[hb], all, p[kb][j], -INFINITY);
-                            add_where<NOT>(acc[hb], all, p[kb][j], NAN);
-                        }
-                    }
-                    acc[hb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, p[kb][j], acc[hb], 0, 0, 0);
-                }
+    Tile<D, KB> tile_of;
+    tile_of.init();
+    const int w0 = wk * KB * 32;  // this wave's keys of a tile
+    if (t0 < t1) {
+        get(t0, smem);
+        put(t0, smem);
     }
+    for (int t = t0; t < t1; ++t) {
+        const u32x4* now = smem + ((t - t0) & 1) * STAGE;
+        u32x4* next = smem + ((t - t0 + 1) & 1) * STAGE;
+        // tile t is there, and nobody reads the other one any more
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (t + 1 < t1) get(t + 1, next);
+        const bool fresh = TREE && t >= ctx_tiles;
+        const int k0 = (fresh ? (t - ctx_tiles) * BN : t * BN) + w0;
+        if (fresh || k0 + KB * 32 - 1 > least) {  // the same in the whole wave
+            const int n = limit - k0 + 1;
+            const unsigned long long seen = fresh ? (k0 < 64 ? nodes >> k0 : 0) : n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1;
+            tile_of.template take<true>(now, now + BN * CPR, qf, w0, c, seen);
+        } else {
+            tile_of.template take<false>(now, now + BN * CPR, qf, w0, c, 0);
+        }
+        if (t + 1 < t1) put(t + 1, next);
+    }
+    auto& acc = tile_of.acc;
+    float m = tile_of.m, l = tile_of.l;
     l = sum_halves(l);
 
     // join the waves that took different keys: each finishes HB / WK of the columns
@@ -454,7 +513,7 @@ __global__ void __launch_bounds__(256) smg_attn_join_t(AttnArgs a) {
 template <bool TREE, bool KV8, int D, int WR>
 int launch_t(const AttnArgs& a, hipStream_t s) {
     constexpr int WK = 4 / WR, KB = WK == 4 ? 1 : 2, BM = 32 * WR;
-    constexpr int tile_bytes = 32 * KB * WK * D * 2 * 2;
+    constexpr int tile_bytes = 32 * KB * WK * D * 2 * 2 * 2;
     constexpr int join_bytes = WK > 1 ? (4 * D / 32 * 16 * WAVE + 8 * WAVE) * 4 : 0;
     constexpr int bytes = tile_bytes > join_bytes ? tile_bytes : join_bytes;
     const long long G = a.H / a.KVH;
