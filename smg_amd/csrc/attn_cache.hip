@@ -27,7 +27,9 @@
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>
 
+#include <atomic>
 #include <cstdint>
+#include <type_traits>
 
 #define WAVE 64
 #define LOG2E 1.44269504088896340736f
@@ -58,9 +60,28 @@ struct AttnArgs {
     long long q_sb, q_st, q_sh, o_sb, o_st, o_sh;        // strides in elements
     long long k_ss, k_sh, k_st, v_ss, v_sh, v_st;
     long long kn_sb, kn_st, kn_sh, vn_sb, vn_st, vn_sh;
-    int B, N, H, KVH, S, T, n_split;
+    int B, N, H, KVH, S, T;
+    int n_split, chunk;          // most splits of a row's keys, and tiles of one
     float scale;
 };
+
+// How a tile of rows shares its key tiles out: runs of `per`, so that long rows have
+// many and short ones one, which writes its result itself.
+struct Runs {
+    int tiles, per, n;
+    __device__ __forceinline__ Runs(const AttnArgs& a, int tiles) : tiles(tiles) {
+        per = max(a.chunk, (tiles + a.n_split - 1) / a.n_split);
+        n = (tiles + per - 1) / per;
+    }
+};
+
+__device__ __forceinline__ int context(const AttnArgs& a, int b, bool tree) {
+    return min(max(a.ctx[b], tree ? 0 : -a.N), a.T);
+}
+// cache rows that the query rows up to `last_row` of a sequence see
+__device__ __forceinline__ int keys_of(const AttnArgs& a, int ctx, int last_row, int G, bool tree) {
+    return tree ? ctx : max(0, min(ctx + last_row / G + 1, a.T));
+}
 
 // max and sum over the two halves of a wave (lane and lane ^ 32)
 __device__ __forceinline__ float max_halves(float x) {
@@ -128,31 +149,48 @@ __device__ __forceinline__ void to_lds(const void* from, u32x4* to) {
                                      (__attribute__((address_space(3))) void*)to, 16, 0, 0);
 }
 
-// a wave's scores, weights and sums over one tile
-template <int D, int KB>
+// A wave's scores, weights and sums.  Addresses in LDS are kept a lane, so that a tile
+// costs one addition each; all else is constant offsets.
+template <int D, int KB, int BN>
 struct Tile {
-    static constexpr int HB = D / 32;
+    static constexpr int HB = D / 32, ROW = D * 2;  // blocks of columns, bytes of a row
+    typedef __attribute__((address_space(3))) const bf16x8* k_ptr;
+    typedef __attribute__((address_space(3))) s16x4* v_ptr;
     f32x16 acc[HB];  // O^T, unnormalised
     float m, mc, l;  // the running maximum, m * c (0 where nothing is seen yet), the sum of this half
+    unsigned k_at[D / 16], v_at[HB];
 
-    __device__ __forceinline__ void init() {
+    // w0: this wave's first key of a tile
+    __device__ __forceinline__ void init(int w0) {
+        const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) k_at[j] = k_chunk<D>(w0 + col, 2 * j + half) * 16;
+        // lane -> key rows r .. r+3 (and, 8 rows on, another 4) of column hb*32 + col
+        const int r = w0 + half * 4 + ((lane & 15) >> 2);
+#pragma unroll
+        for (int hb = 0; hb < HB; ++hb)
+            v_at[hb] = BN * ROW + v_chunk<D>(r, hb * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) * 16 + (lane & 1) * 8;
 #pragma unroll
         for (int i = 0; i < HB; ++i) acc[i] = (f32x16)0.f;
         m = -INFINITY;
         mc = l = 0.f;
     }
-    // keys w0 .. w0 + 32 KB - 1 of the tile; where MASKED, bit i of `seen` is key i of those
+    // this wave's 32 KB keys of the tile at `at`; where MASKED, bit i of `seen` is key i of those
     template <bool MASKED>
-    __device__ __forceinline__ void take(const u32x4* sk, const u32x4* sv, const bf16x8* qf, int w0, float c, unsigned long long seen) {
+    __device__ __forceinline__ void take(unsigned at, const bf16x8* qf, float c, unsigned long long seen) {
         const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+        // K a block of 32 keys ahead of the products
         f32x16 s[KB];
+        bf16x8 kf[D / 16];
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) kf[j] = *(k_ptr)(size_t)(k_at[j] + at);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
             s[kb] = (f32x16)0.f;
 #pragma unroll
             for (int j = 0; j < D / 16; ++j) {
-                const bf16x8 kf = __builtin_bit_cast(bf16x8, sk[k_chunk<D>(w0 + kb * 32 + col, 2 * j + half)]);
-                s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[j], s[kb], 0, 0, 0);
+                s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[j], qf[j], s[kb], 0, 0, 0);
+                if (kb + 1 < KB) kf[j] = *(k_ptr)(size_t)(k_at[j] + at + (kb + 1) * 32 * ROW);
             }
         }
         float top = -INFINITY;
@@ -193,14 +231,9 @@ struct Tile {
             for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int hb = 0; hb < HB; ++hb) {
-                    // lane -> key rows r0 .. r0+3 (and r0+8 ..) of column hb*32 + col
-                    const int r0 = w0 + kb * 32 + j * 16 + half * 4 + ((lane & 15) >> 2);
-                    const int cc = hb * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
-                    typedef __attribute__((address_space(3))) s16x4* lds_t;
-                    const char* lo = (const char*)&sv[v_chunk<D>(r0, cc)] + (lane & 1) * 8;
-                    const char* hi = (const char*)&sv[v_chunk<D>(r0 + 8, cc)] + (lane & 1) * 8;
-                    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)lo);
-                    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)hi);
+                    const unsigned v = v_at[hb] + at + (kb * 32 + j * 16) * ROW;
+                    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v_ptr)(size_t)v);
+                    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v_ptr)(size_t)(v + 8 * ROW));
                     bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
                     if (MASKED) {
                         // 0 * inf is NaN: a masked key's weight is 0, but its V must not
@@ -225,19 +258,31 @@ struct Tile {
 };
 
 // TREE: drafted nodes with their own K/V after the context.  KV8: e4m3 cache.
-// WR waves share the query rows of a tile (32 each), WK = 4 / WR split its keys.
+// WR waves share the query rows of a tile (32 each), WK of them split its keys.
 template <bool TREE, bool KV8, int D, int WR>
-__global__ void __launch_bounds__(256, WR == 4 ? 2 : 1) smg_attn_cache_t(AttnArgs a) {
-    constexpr int WK = 4 / WR;
-    constexpr int KB = WK == 4 ? 1 : 2;      // blocks of 32 keys a wave takes of a tile
-    constexpr int BN = 32 * KB * WK;         // keys of a tile
-    constexpr int BM = 32 * WR;              // query rows of a workgroup
+struct Shape {
+    static constexpr int WK = KV8 ? (WR == 8 ? 1 : 2) : 4 / WR;
+    static constexpr int WAVES = WR * WK;
+    static constexpr int THREADS = WAVES * WAVE;
+    static constexpr int KB = WK == 1 ? 2 : 1;     // blocks of 32 keys a wave takes of a tile
+    static constexpr int BN = 32 * KB * WK;        // keys of a tile
+    static constexpr int BM = 32 * WR;             // query rows of a workgroup
+    static constexpr int TILE = 2 * BN * (D / 8);  // 16-byte chunks of a tile, K then V
+    static constexpr int RAW = TILE / 2;           // the same in 8 bits
+    static constexpr int RAWS = 3;
+    static constexpr int CHUNKS = 2 * TILE + (KV8 ? RAWS * RAW + (TREE ? TILE : 0) : 0);
+    static constexpr int WAVES_A_SIMD = KV8 && WR == 2 ? 1 : WR == 1 ? 1 : 2;
+};
+
+template <bool TREE, bool KV8, int D, int WR>
+__global__ void __launch_bounds__((Shape<TREE, KV8, D, WR>::THREADS), (Shape<TREE, KV8, D, WR>::WAVES_A_SIMD)) smg_attn_cache_t(AttnArgs a) {
+    using Z = Shape<TREE, KV8, D, WR>;
+    constexpr int WK = Z::WK, KB = Z::KB, BN = Z::BN, BM = Z::BM, WAVES = Z::WAVES, THREADS = Z::THREADS;
     constexpr int CPR = D / 8;               // 16-byte chunks a row
     constexpr int HB = D / 32;
-    constexpr int STAGE = 2 * BN * CPR;      // chunks of a tile, K then V; two tiles in turn
     extern __shared__ u32x4 smem[];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wave % WR, wk = wave / WR;
     const int half = lane >> 5, col = lane & 31;
     const int G = a.H / a.KVH;
@@ -276,18 +321,27 @@ __global__ void __launch_bounds__(256, WR == 4 ? 2 : 1) smg_attn_cache_t(AttnArg
             if (found) {
                 const int l = __ffsll((long long)found) - 1;
                 b = b0 + l;
-                base = __shfl(lo, l, WAVE);
-                rows = (__shfl(hi, l, WAVE) - base) * G;
-                row0 = (tile - before - __shfl(sum - n, l, WAVE)) * BM;
+                base = __builtin_amdgcn_readlane(lo, l);
+                rows = (__builtin_amdgcn_readlane(hi, l) - base) * G;
+                row0 = (tile - before - __builtin_amdgcn_readlane(sum - n, l)) * BM;
                 break;
             }
-            before += __shfl(sum, WAVE - 1, WAVE);
+            before += __builtin_amdgcn_readlane(sum, WAVE - 1);
         }
         if (b < 0) return;
     }
     const int slot = a.slots[b];
     const bool cached = slot >= 0 && slot < a.S;
-    const int ctx = min(max(a.ctx[b], TREE ? 0 : -a.N), a.T);
+    const int ctx = context(a, b, TREE);
+
+    // keys of the workgroup, in tiles; a split takes a run of them
+    const int last_row = min(row0 + BM, rows) - 1;
+    const int kend = cached ? keys_of(a, ctx, last_row, G, TREE) : 0;
+    const int ctx_tiles = (kend + BN - 1) / BN;
+    const int new_tiles = TREE ? (a.N + BN - 1) / BN : 0;
+    const Runs runs(a, cached ? ctx_tiles + new_tiles : 0);
+    if (split > 0 && split >= runs.n) return;
+    const int t0 = split * runs.per, t1 = min(runs.tiles, t0 + runs.per);
 
     // this lane's query row, and the last cache row that it sees
     const int row = row0 + wr * 32 + col;
@@ -322,103 +376,166 @@ __global__ void __launch_bounds__(256, WR == 4 ? 2 : 1) smg_attn_cache_t(AttnArg
         limit = live && cached ? min(ctx + token, a.T - 1) : -1;
     }
 
-    // keys of the workgroup, in tiles; a split takes a run of them
-    const int last_row = min(row0 + BM, rows) - 1;
-    const int kend = !cached ? 0 : TREE ? ctx : max(0, min(ctx + last_row / G + 1, a.T));
-    const int ctx_tiles = (kend + BN - 1) / BN;
-    const int new_tiles = TREE ? (a.N + BN - 1) / BN : 0;
-    const int tiles = ctx_tiles + (cached ? new_tiles : 0);
-    const int per_split = (tiles + a.n_split - 1) / a.n_split;
-    const int t0 = split * per_split, t1 = min(tiles, t0 + per_split);
     const size_t unit = KV8 ? 1 : 2;
     const char* kbase = (const char*)a.k + (cached ? slot * a.k_ss + kvh * a.k_sh : 0) * unit;
     const char* vbase = (const char*)a.v + (cached ? slot * a.v_ss + kvh * a.v_sh : 0) * unit;
     const __hip_bfloat16* knew = TREE ? a.k_new + b * a.kn_sb + kvh * a.kn_sh : nullptr;
     const __hip_bfloat16* vnew = TREE ? a.v_new + b * a.vn_sb + kvh * a.vn_sh : nullptr;
     const float c = a.scale * LOG2E;
-    // rows of this wave that see every key of a tile need no mask
-    int least = live ? limit : 0x7fffffff;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) least = min(least, __shfl_xor(least, o, WAVE));
-    least = __builtin_amdgcn_readfirstlane(least);
+    // Tiles whose every key every row sees (nodes outside the tree get their zeros at
+    // the end) need no mask.  They come first, and in a loop of their own: one loop
+    // that chooses would move the accumulators about.
+    const int full = min(t1, (TREE ? kend : max(0, min(ctx + row0 / G + 1, kend))) / BN);
 
-    // Tile t to LDS: 16-bit rows straight from memory, permuted by where each lane
-    // reads; an 8-bit cache's by way of registers (`put` widens them later).
-    constexpr int PER = BN * CPR / 256;  // chunks a thread
-    constexpr int RPI = 64 / CPR;        // rows of a wave's 1 KB
-    uint2 k8[KV8 ? PER : 1], v8[KV8 ? PER : 1];
-    auto get = [&](int t, u32x4* to) {
-        const bool fresh = TREE && t >= ctx_tiles;
-        const int n0 = fresh ? (t - ctx_tiles) * BN : t * BN;
-        const int nlast = (fresh ? a.N : kend) - 1;  // rows past the end repeat the last
-        if (KV8 && !fresh) {
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const int at = i * 256 + tid;
-                const long long src = min(n0 + at / CPR, nlast);
-                k8[i] = *(const uint2*)(kbase + src * a.k_st + at % CPR * 8);
-                v8[i] = *(const uint2*)(vbase + src * a.v_st + at % CPR * 8);
-            }
-        } else {
-            const __hip_bfloat16* kp = fresh ? knew : (const __hip_bfloat16*)kbase;
-            const __hip_bfloat16* vp = fresh ? vnew : (const __hip_bfloat16*)vbase;
-            const long long ks = fresh ? a.kn_st : a.k_st, vs = fresh ? a.vn_st : a.v_st;
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const int r0 = (i * 4 + wave) * RPI, r = r0 + lane / CPR, cc = lane % CPR;
-                const long long src = min(n0 + r, nlast);
-                to_lds(kp + src * ks + (cc ^ (r & (CPR - 1))) * 8, to + r0 * CPR);
-                to_lds(vp + src * vs + (cc ^ v_swap<D>(r)) * 8, to + BN * CPR + r0 * CPR);
-            }
-        }
-    };
-    auto put = [&](int t, u32x4* to) {
-        if (!KV8 || (TREE && t >= ctx_tiles)) return;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int r = (i * 256 + tid) / CPR, cc = tid % CPR;
-            to[k_chunk<D>(r, cc)] = u32x4{fp8x2_to_bf16x2(k8[i].x, false), fp8x2_to_bf16x2(k8[i].x, true),
-                                          fp8x2_to_bf16x2(k8[i].y, false), fp8x2_to_bf16x2(k8[i].y, true)};
-            to[BN * CPR + v_chunk<D>(r, cc)] = u32x4{fp8x2_to_bf16x2(v8[i].x, false), fp8x2_to_bf16x2(v8[i].x, true),
-                                                     fp8x2_to_bf16x2(v8[i].y, false), fp8x2_to_bf16x2(v8[i].y, true)};
-        }
-    };
-
-    Tile<D, KB> tile_of;
-    tile_of.init();
     const int w0 = wk * KB * 32;  // this wave's keys of a tile
-    if (t0 < t1) {
-        get(t0, smem);
-        put(t0, smem);
-    }
-    for (int t = t0; t < t1; ++t) {
-        const u32x4* now = smem + ((t - t0) & 1) * STAGE;
-        u32x4* next = smem + ((t - t0 + 1) & 1) * STAGE;
-        // tile t is there, and nobody reads the other one any more
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (t + 1 < t1) get(t + 1, next);
-        const bool fresh = TREE && t >= ctx_tiles;
-        const int k0 = (fresh ? (t - ctx_tiles) * BN : t * BN) + w0;
-        if (fresh || k0 + KB * 32 - 1 > least) {  // the same in the whole wave
-            const int n = limit - k0 + 1;
+    Tile<D, KB, BN> tile_of;
+    tile_of.init(w0);
+    const unsigned lds = (unsigned)(size_t)(__attribute__((address_space(3))) void*)smem;
+    // tile t from LDS: of the cache, or of the drafted nodes after it
+    auto take = [&](int t, int chunk, auto masked) {
+        const unsigned now = lds + chunk * 16;
+        if constexpr (decltype(masked)::value) {
+            const bool fresh = TREE && t >= ctx_tiles;
+            const int k0 = (fresh ? (t - ctx_tiles) * BN : t * BN) + w0, n = limit - k0 + 1;
             const unsigned long long seen = fresh ? (k0 < 64 ? nodes >> k0 : 0) : n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1;
-            tile_of.template take<true>(now, now + BN * CPR, qf, w0, c, seen);
+            tile_of.template take<true>(now, qf, c, seen);
         } else {
-            tile_of.template take<false>(now, now + BN * CPR, qf, w0, c, 0);
+            tile_of.template take<false>(now, qf, c, 0);
         }
-        if (t + 1 < t1) put(t + 1, next);
+    };
+    const std::true_type masked;
+    const std::false_type whole;
+    // 16-bit rows n0 .. n0 + BN - 1 to LDS, permuted by where each lane reads; rows
+    // past the end repeat the last.  A whole tile takes a lane's fixed offsets from
+    // addresses that the wave shares (the permutation repeats every 16 rows).
+    auto rows_to_lds = [&](const __hip_bfloat16* kp, const __hip_bfloat16* vp, long long ks, long long vs, int n0, int nlast, u32x4* to) {
+        constexpr int RPI = WAVE / CPR, STEP = RPI * WAVES;  // rows of a wave's 1 KB, of all waves' ones
+        static_assert(STEP % (D == 128 ? 16 : 8) == 0, "the permutation repeats");
+        const int r0 = wave * RPI + lane / CPR, cc = lane % CPR;
+        const int kc = (cc ^ (r0 & (CPR - 1))) * 8, vc = (cc ^ v_swap<D>(r0)) * 8;
+        if (n0 + BN - 1 <= nlast && max(ks, vs) < (1 << 20) && min(ks, vs) >= 0) {
+            const unsigned ko = (unsigned)(r0 * (int)ks + kc) * 2, vo = (unsigned)(r0 * (int)vs + vc) * 2;
+#pragma unroll
+            for (int i = 0; i < BN / STEP; ++i) {
+                to_lds((const char*)(kp + (n0 + i * STEP) * ks) + ko, to + (i * STEP + wave * RPI) * CPR);
+                to_lds((const char*)(vp + (n0 + i * STEP) * vs) + vo, to + (BN + i * STEP + wave * RPI) * CPR);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < BN / STEP; ++i) {
+                const long long src = min(n0 + i * STEP + r0, nlast);
+                to_lds(kp + src * ks + kc, to + (i * STEP + wave * RPI) * CPR);
+                to_lds(vp + src * vs + vc, to + (BN + i * STEP + wave * RPI) * CPR);
+            }
+        }
+    };
+    if constexpr (!KV8) {
+        // two tiles in turn: one on its way while the other is computed
+        auto get = [&](int t, u32x4* to) {
+            if (TREE && t >= ctx_tiles)
+                rows_to_lds(knew, vnew, a.kn_st, a.vn_st, (t - ctx_tiles) * BN, a.N - 1, to);
+            else
+                rows_to_lds((const __hip_bfloat16*)kbase, (const __hip_bfloat16*)vbase, a.k_st, a.v_st, t * BN, kend - 1, to);
+        };
+        auto step = [&](int t, auto mask) {
+            // tile t is there, and nobody reads the one before it any more
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            if (t + 1 < t1) get(t + 1, smem + ((t - t0 + 1) & 1) * Z::TILE);
+            take(t, ((t - t0) & 1) * Z::TILE, mask);
+        };
+        if (t0 < t1) get(t0, smem);
+        int t = t0;
+        for (; t < full; ++t) step(t, whole);
+        for (; t < t1; ++t) step(t, masked);
+    } else {
+        // 8-bit tiles come as they are, up to three on their way (memory is what the
+        // long ones wait for), and the workgroup widens one while it computes the one
+        // before it.  The drafted nodes' tile has a place of its own.
+        constexpr int UPR = D / 16;                     // 16-byte units a row
+        constexpr int PER = 2 * BN * UPR / THREADS;     // units a thread, of K then V
+        u32x4* raws = smem + 2 * Z::TILE;
+        u32x4* drafts = raws + Z::RAWS * Z::RAW;
+        const int tc = min(t1, ctx_tiles);              // the cache's tiles end here
+        auto get = [&](int t) {
+            u32x4* to = raws + t % Z::RAWS * Z::RAW;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int u0 = (i * WAVES + wave) * WAVE;
+                const bool v = u0 >= BN * UPR;
+                const int r0 = (u0 - (v ? BN * UPR : 0)) / UPR;  // the wave's first row of 64 / UPR
+                const char* from = v ? vbase : kbase;
+                const long long st = v ? a.v_st : a.k_st;
+                if (t * BN + BN <= kend && st < (1 << 20) && st >= 0)
+                    to_lds(from + (t * BN + r0) * st + (unsigned)(lane / UPR * (int)st + lane % UPR * 16), to + u0);
+                else
+                    to_lds(from + (long long)min(t * BN + r0 + lane / UPR, kend - 1) * st + lane % UPR * 16, to + u0);
+            }
+        };
+        auto widen = [&](int t) {
+            const u32x4* from = raws + t % Z::RAWS * Z::RAW;
+            u32x4* to = smem + (t & 1) * Z::TILE;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int u = i * THREADS + tid, r = u / UPR % BN, cc = u % UPR * 2;
+                const bool v = u >= BN * UPR;
+                const u32x4 x = from[u];
+                const u32x4 lo = {fp8x2_to_bf16x2(x[0], false), fp8x2_to_bf16x2(x[0], true), fp8x2_to_bf16x2(x[1], false), fp8x2_to_bf16x2(x[1], true)};
+                const u32x4 hi = {fp8x2_to_bf16x2(x[2], false), fp8x2_to_bf16x2(x[2], true), fp8x2_to_bf16x2(x[3], false), fp8x2_to_bf16x2(x[3], true)};
+                to[v ? BN * CPR + v_chunk<D>(r, cc) : k_chunk<D>(r, cc)] = lo;
+                to[v ? BN * CPR + v_chunk<D>(r, cc + 1) : k_chunk<D>(r, cc + 1)] = hi;
+            }
+        };
+        static_assert(BN == 64, "one tile of drafted nodes");
+        if (TREE && t1 > ctx_tiles) rows_to_lds(knew, vnew, a.kn_st, a.vn_st, 0, a.N - 1, drafts);
+#pragma unroll
+        for (int i = 0; i < Z::RAWS; ++i)
+            if (t0 + i < tc) get(t0 + i);
+        if (t0 < tc) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            widen(t0);
+        }
+        auto step = [&](int t, auto mask) {
+            // this wave's part of raw tile t + 1 is there (t + 2 may be on its way) and
+            // its part of tile t is widened: after the barrier, all are
+            if (t + 2 < tc)
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(PER) : "memory");
+            else
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            if (t + Z::RAWS < tc) get(t + Z::RAWS);  // where raw tile t was
+            if (t + 1 < tc) widen(t + 1);            // where tile t - 1 was
+            take(t, (t & 1) * Z::TILE, mask);
+        };
+        int t = t0;
+        for (; t < full; ++t) step(t, whole);
+        for (; t < tc; ++t) step(t, masked);
+        if (TREE && t1 > ctx_tiles) {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            take(ctx_tiles, (int)(drafts - smem), masked);
+        }
     }
     auto& acc = tile_of.acc;
     float m = tile_of.m, l = tile_of.l;
     l = sum_halves(l);
+    if (TREE && !nodes) {
+        m = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int i = 0; i < HB; ++i) acc[i] = (f32x16)0.f;
+    }
 
     // join the waves that took different keys: each finishes HB / WK of the columns
     constexpr int HW = HB / WK;  // WK <= HB
     if constexpr (WK > 1) {
-        float* so = (float*)smem;                     // [4][HB * 16][64]
-        float* sm = so + 4 * HB * 16 * WAVE;          // [4][2][64]
+        float* so = (float*)smem;                     // [WAVES][HB * 16][64]
+        float* sm = so + WAVES * HB * 16 * WAVE;      // [WAVES][2][64]
         __syncthreads();
 #pragma unroll
         for (int hb = 0; hb < HB; ++hb)
@@ -451,7 +568,7 @@ __global__ void __launch_bounds__(256, WR == 4 ? 2 : 1) smg_attn_cache_t(AttnArg
     }
     if (!live) return;
     const int hb0 = WK > 1 ? wk * HW : 0;
-    if (a.n_split > 1) {
+    if (runs.n > 1) {
         const size_t all_rows = (size_t)(TREE ? a.B * (long long)a.N : a.N);
         const size_t at = ((size_t)split * all_rows + (TREE ? (size_t)b * a.N : base) + token) * a.H + head;
 #pragma unroll
@@ -466,7 +583,8 @@ __global__ void __launch_bounds__(256, WR == 4 ? 2 : 1) smg_attn_cache_t(AttnArg
         }
         return;
     }
-    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // no key seen: zeros; NaN stays
+    // no key seen: zeros; NaN stays
+    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
     __hip_bfloat16* op = a.out + (TREE ? b * a.o_sb : 0) + (base + token) * a.o_st + head * a.o_sh;
 #pragma unroll
     for (int hb = 0; hb < HW; ++hb)
@@ -479,74 +597,131 @@ __global__ void __launch_bounds__(256, WR == 4 ? 2 : 1) smg_attn_cache_t(AttnArg
         }
 }
 
-// Joins the splits of a row: out = sum_s 2^((m_s - m) c) O_s / sum_s 2^((m_s - m) c) l_s.
-// One wave a (token, head).
+// Joins the runs of a row that has several:
+//   out = sum_s 2^((m_s - m) c) O_s / sum_s 2^((m_s - m) c) l_s.
+// A workgroup has a (token, head), and each of its four waves every fourth load, which
+// covers 4 * 64 / D runs: all of a row's loads are on their way at once.
 template <bool TREE, int D>
-__global__ void __launch_bounds__(256) smg_attn_join_t(AttnArgs a) {
-    const int lane = threadIdx.x & 63;
+__global__ void __launch_bounds__(256) smg_attn_join_t(AttnArgs a, int BM, int BN) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const long long all_rows = TREE ? a.B * (long long)a.N : a.N;
-    const long long rh = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (rh >= all_rows * a.H) return;
+    const long long rh = blockIdx.x;
     const long long r = rh / a.H;
-    const int h = (int)(rh % a.H);
-    if constexpr (!TREE) {  // rows that no sequence covers stay as they are
-        if (r < max(a.cu[0], 0) || r >= a.cu[a.B]) return;
+    const int h = (int)(rh % a.H), G = a.H / a.KVH;
+    int b, rows, token;
+    if constexpr (TREE) {
+        b = (int)(r / a.N);
+        token = (int)(r % a.N);
+        rows = a.N * G;
+    } else {
+        // the last sequence that starts at r or before; rows outside all stay
+        if (r < a.cu[0] || r >= a.cu[a.B]) return;
+        int lo = 0, hi = a.B;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (a.cu[mid] <= r)
+                lo = mid;
+            else
+                hi = mid;
+        }
+        b = lo;
+        const int first = max(a.cu[b], 0);
+        token = (int)r - first;
+        rows = (min(a.cu[b + 1], a.N) - first) * G;
     }
+    const int slot = a.slots[b];
+    if (slot < 0 || slot >= a.S) return;
+    const int last_row = min((token * G + h % G) / BM * BM + BM, rows) - 1;
+    const int kend = keys_of(a, context(a, b, TREE), last_row, G, TREE);
+    const int n = Runs(a, (kend + BN - 1) / BN + (TREE ? (a.N + BN - 1) / BN : 0)).n;
+    if (n <= 1) return;
+    // a lane a run (at most 64 of them)
     const float c = a.scale * LOG2E;
-    constexpr int E = D / WAVE;
-    float top = -INFINITY, sum = 0.f, o[E] = {};
-    for (int s = 0; s < a.n_split; ++s) top = fmaxf(top, a.part_ml[(s * all_rows * a.H + rh) * 2]);
-    for (int s = 0; s < a.n_split; ++s) {
-        const size_t at = s * all_rows * a.H + rh;
-        const float ms = a.part_ml[at * 2];
-        const float f = ms == -INFINITY ? 0.f : exp2f((ms - top) * c);
-        sum += f * a.part_ml[at * 2 + 1];
+    const size_t run = all_rows * a.H;
+    float ms = -INFINITY, ls = 0.f;
+    if (lane < n) ms = a.part_ml[(lane * run + rh) * 2], ls = a.part_ml[(lane * run + rh) * 2 + 1];
+    constexpr int LPR = D / 4, RPL = WAVE / LPR;  // lanes of a row, rows of a load
+    const int e = lane % LPR * 4;
+    f32x4 part[WAVE / 4 / RPL];
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] += f * a.part_o[at * D + lane * E + e];
+    for (int i = 0; i < WAVE / 4 / RPL; ++i) {
+        const int s = (i * 4 + wave) * RPL + lane / LPR;
+        part[i] = s < n ? *(const f32x4*)(a.part_o + (s * run + rh) * D + e) : (f32x4)0.f;
     }
-    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-    __hip_bfloat16* op = TREE ? a.out + r / a.N * a.o_sb + r % a.N * a.o_st : a.out + r * a.o_st;
+    float top = ms;
 #pragma unroll
-    for (int e = 0; e < E; ++e) op[h * a.o_sh + lane * E + e] = (__hip_bfloat16)(o[e] * inv);
+    for (int o = 1; o < WAVE; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, WAVE));
+    const float fs = ms == -INFINITY ? 0.f : exp2f((ms - top) * c);
+    float sum = fs * ls;
+#pragma unroll
+    for (int o = 1; o < WAVE; o <<= 1) sum += __shfl_xor(sum, o, WAVE);
+    f32x4 o = 0.f;
+#pragma unroll
+    for (int i = 0; i < WAVE / 4 / RPL; ++i) o += __shfl(fs, (i * 4 + wave) * RPL + lane / LPR, WAVE) * part[i];
+    __shared__ f32x4 rest[4][WAVE];
+    rest[wave][lane] = o;
+    __syncthreads();
+    if (threadIdx.x >= LPR) return;
+    o = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4 * RPL; ++i) o += rest[i / RPL][i % RPL * LPR + lane];
+    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+    __hip_bfloat16* op = (TREE ? a.out + b * a.o_sb + token * a.o_st : a.out + r * a.o_st) + h * a.o_sh + e;
+    bf16x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = (__bf16)(o[i] * inv);
+    *(bf16x4*)op = w;
 }
 
 template <bool TREE, bool KV8, int D, int WR>
-int launch_t(const AttnArgs& a, hipStream_t s) {
-    constexpr int WK = 4 / WR, KB = WK == 4 ? 1 : 2, BM = 32 * WR;
-    constexpr int tile_bytes = 32 * KB * WK * D * 2 * 2 * 2;
-    constexpr int join_bytes = WK > 1 ? (4 * D / 32 * 16 * WAVE + 8 * WAVE) * 4 : 0;
+int launch_t(AttnArgs a, int chunk_keys, hipStream_t s) {
+    using Z = Shape<TREE, KV8, D, WR>;
+    constexpr int BM = Z::BM, BN = Z::BN;
+    constexpr int tile_bytes = Z::CHUNKS * 16;
+    constexpr int join_bytes = Z::WK > 1 ? Z::WAVES * (D / 32 * 16 + 2) * WAVE * 4 : 0;
     constexpr int bytes = tile_bytes > join_bytes ? tile_bytes : join_bytes;
+    static_assert(bytes <= 160 * 1024, "LDS of a compute unit");
     const long long G = a.H / a.KVH;
     const long long tiles = TREE ? a.B * ((a.N * G + BM - 1) / BM) : a.N * G / BM + a.B;
     const long long grid = tiles * a.KVH;
-    if (grid > 0x7fffffffll || a.n_split > 65535) return -5;
-    static bool set = false;  // more dynamic LDS than the default limit
-    if (!set) {
+    a.chunk = (chunk_keys + BN - 1) / BN;
+    if (grid > 0x7fffffffll || a.n_split > WAVE) return -5;
+    // more dynamic LDS than the default limit, once a device
+    static std::atomic<unsigned long long> set{0};
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return -2;
+    if (dev > 63 || !(set.load(std::memory_order_relaxed) >> dev & 1)) {
         if (hipFuncSetAttribute((const void*)smg_attn_cache_t<TREE, KV8, D, WR>,
                                 hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
             return -2;
-        set = true;
+        if (dev <= 63) set.fetch_or(1ull << dev, std::memory_order_relaxed);
     }
-    hipLaunchKernelGGL((smg_attn_cache_t<TREE, KV8, D, WR>), dim3((unsigned)grid, a.n_split), dim3(256), bytes, s, a);
+    hipLaunchKernelGGL((smg_attn_cache_t<TREE, KV8, D, WR>), dim3((unsigned)grid, a.n_split), dim3(Z::THREADS), bytes, s, a);
     if (a.n_split > 1) {
         const long long rh = (TREE ? a.B * (long long)a.N : a.N) * a.H;
-        hipLaunchKernelGGL((smg_attn_join_t<TREE, D>), dim3((unsigned)((rh + 3) / 4)), dim3(256), 0, s, a);
+        if (rh > 0x7fffffffll) return -5;
+        hipLaunchKernelGGL((smg_attn_join_t<TREE, D>), dim3((unsigned)rh), dim3(256), 0, s, a, BM, BN);
     }
     return hipGetLastError() == hipSuccess ? 0 : -2;
 }
 
+template <bool TREE, bool KV8, int D>
+int launch_d(const AttnArgs& a, int wr, int chunk, hipStream_t s) {
+    if constexpr (KV8) {
+        if (wr <= 2) return launch_t<TREE, true, D, 2>(a, chunk, s);
+        if (wr == 4) return launch_t<TREE, true, D, 4>(a, chunk, s);
+        return launch_t<TREE, true, D, 8>(a, chunk, s);
+    } else {
+        if constexpr (D == 128)
+            if (wr == 1) return launch_t<TREE, false, D, 1>(a, chunk, s);
+        if (wr <= 2) return launch_t<TREE, false, D, 2>(a, chunk, s);
+        return launch_t<TREE, false, D, 4>(a, chunk, s);
+    }
+}
+
 template <bool TREE, bool KV8>
-int launch(const AttnArgs& a, int D, int wr, hipStream_t s) {
-    if (D == 128) {
-        if (wr == 1) return launch_t<TREE, KV8, 128, 1>(a, s);
-        if (wr == 2) return launch_t<TREE, KV8, 128, 2>(a, s);
-        return launch_t<TREE, KV8, 128, 4>(a, s);
-    }
-    if (D == 64) {
-        if (wr <= 2) return launch_t<TREE, KV8, 64, 2>(a, s);
-        return launch_t<TREE, KV8, 64, 4>(a, s);
-    }
-    return -1;
+int launch(const AttnArgs& a, int D, int wr, int chunk, hipStream_t s) {
+    return D == 128 ? launch_d<TREE, KV8, 128>(a, wr, chunk, s) : D == 64 ? launch_d<TREE, KV8, 64>(a, wr, chunk, s) : -1;
 }
 
 int bad_shape(int H, int KVH, int S, int T, int n_split) {
@@ -561,8 +736,9 @@ int bad_shape(int H, int KVH, int S, int T, int n_split) {
 extern "C" int smg_attn_prefill_launch(
     const void* q, const void* k, const void* v, const void* slots, const void* ctx, const void* cu,
     void* out, void* part_o, void* part_ml, const long long* strides, int B, int N, int H, int KVH,
-    int S, int T, int D, int n_split, int wr, float scale, int kv_fp8, void* stream) {
+    int S, int T, int D, int n_split, int chunk, int wr, float scale, int kv_fp8, void* stream) {
     if (int rc = bad_shape(H, KVH, S, T, n_split)) return rc;
+    if (chunk < 1) return -3;
     if (B < 1 || N < 1) return 0;
     AttnArgs a = {};
     a.q = (const __hip_bfloat16*)q;
@@ -579,17 +755,18 @@ extern "C" int smg_attn_prefill_launch(
     a.v_ss = strides[7], a.v_sh = strides[8], a.v_st = strides[9];
     a.B = B, a.N = N, a.H = H, a.KVH = KVH, a.S = S, a.T = T, a.n_split = n_split;
     a.scale = scale;
-    return kv_fp8 ? launch<false, true>(a, D, wr, (hipStream_t)stream)
-                  : launch<false, false>(a, D, wr, (hipStream_t)stream);
+    return kv_fp8 ? launch<false, true>(a, D, wr, chunk, (hipStream_t)stream)
+                  : launch<false, false>(a, D, wr, chunk, (hipStream_t)stream);
 }
 
 // strides: q batch/token/head, out batch/token/head, k and v as above, k_new and v_new batch/token/head
 extern "C" int smg_attn_tree_launch(
     const void* q, const void* k_new, const void* v_new, const void* k, const void* v,
     const void* slots, const void* ctx, const void* parents, void* out, void* part_o, void* part_ml,
-    const long long* strides, int B, int N, int H, int KVH, int S, int T, int D, int n_split, int wr,
-    float scale, int kv_fp8, void* stream) {
+    const long long* strides, int B, int N, int H, int KVH, int S, int T, int D, int n_split,
+    int chunk, int wr, float scale, int kv_fp8, void* stream) {
     if (int rc = bad_shape(H, KVH, S, T, n_split)) return rc;
+    if (chunk < 1) return -3;
     if (N > 64) return -3;
     if (B < 1 || N < 1) return 0;
     AttnArgs a = {};
@@ -612,6 +789,6 @@ extern "C" int smg_attn_tree_launch(
     a.vn_sb = strides[15], a.vn_st = strides[16], a.vn_sh = strides[17];
     a.B = B, a.N = N, a.H = H, a.KVH = KVH, a.S = S, a.T = T, a.n_split = n_split;
     a.scale = scale;
-    return kv_fp8 ? launch<true, true>(a, D, wr, (hipStream_t)stream)
-                  : launch<true, false>(a, D, wr, (hipStream_t)stream);
+    return kv_fp8 ? launch<true, true>(a, D, wr, chunk, (hipStream_t)stream)
+                  : launch<true, false>(a, D, wr, chunk, (hipStream_t)stream);
 }

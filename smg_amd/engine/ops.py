@@ -7,7 +7,7 @@ to the host, so all of them can be captured into graphs.
 The cache is the engine's: [slots, kv heads, positions, head dim] a layer, in
 bfloat16 or float8_e4m3fn; its dimensions may have any strides but the last,
 which is dense.  Rows of tensors that kernels read 16 bytes at a time start at
-multiples of 16 bytes.
+multiples of 16 bytes (8 where tree_commit writes an 8-bit cache).
 
 What the host cannot see is bounded on the device: a sequence whose slot lies
 outside the cache is a padding entry, lengths and offsets are cut to the tensors.
@@ -45,12 +45,11 @@ def _check(name: str, t, dtypes: tuple, dim: int, dev: Optional[int]) -> None:
     raise ValueError(f"{name} is on {t.device}, the other tensors are not")
 
 
-def _rows(name: str, t: torch.Tensor) -> tuple:
+def _rows(name: str, t: torch.Tensor, unit: int = 16) -> tuple:
     """The strides but the last, of a tensor that is dense in its last dimension and
-    whose rows start at multiples of 16 bytes (8 in an 8-bit cache)."""
+    whose rows start at multiples of `unit` bytes."""
     strides = t.stride()
     e = t.element_size()
-    unit = 16 if e > 1 else 8
     at = t.data_ptr()
     for s in strides[:-1]:
         at |= s * e
@@ -120,15 +119,17 @@ def _launch(kernel, dev: int, *args) -> None:
             kernel(*args, stream)
 
 
-def _plan(rows: int, seqs: int, total: int, ctx: int, KVH: int, D: int) -> Tuple[int, int]:
-    """(waves along the query rows, splits of the keys) for `seqs` sequences of about
-    `rows` rows a kv head, `total` in all, and up to `ctx` keys."""
-    wr = 1 if rows <= 32 and D == 128 else 2 if rows <= 64 else 4
-    work = (total // (32 * wr) + seqs) * KVH
-    split = 1
-    while split < 64 and work * split < 512 and ctx >= split * 512:
-        split *= 2
-    return wr, split
+_WORK = 512  # workgroups that fill the card, where rows alone give fewer
+
+
+def _plan(rows: int, tiles, ctx: int, KVH: int, D: int, fp8: bool) -> Tuple[int, int, int]:
+    """(waves along the query rows, most splits of the keys, keys of a split) for
+    sequences of about `rows` rows a kv head and up to `ctx` keys; tiles(rows of a
+    tile) is how many tiles of rows there are."""
+    wr = 1 if rows <= 32 and D == 128 and not fp8 else 2 if rows <= 64 else 8 if fp8 and rows > 128 else 4
+    work = tiles(32 * wr) * KVH
+    split = 1 if work >= 256 else max(1, min(_WORK // work, ctx // 256, 64))
+    return wr, split, -(-ctx // split)
 
 
 def _parts(split: int, rows: int, D: int, q: torch.Tensor) -> tuple:
@@ -171,11 +172,11 @@ def attn_prefill(
         return out
     total = N * (H // KVH)
     ctx = T if max_ctx is None else max(1, min(int(max_ctx), T))
-    wr, split = _plan(total // B, B, total, ctx, KVH, D)
+    wr, split, chunk = _plan(total // B, lambda bm: total // bm + B, ctx, KVH, D, k_cache.dtype is _FP8)
     part, po, pm = _parts(split, N * H, D, q)
     _launch(
         _core.attn_prefill, dev, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), p_slots, p_starts, p_cu,
-        out.data_ptr(), po, pm, strides, B, N, H, KVH, S, T, D, split, wr, scale, k_cache.dtype is _FP8,
+        out.data_ptr(), po, pm, strides, B, N, H, KVH, S, T, D, split, chunk, wr, scale, k_cache.dtype is _FP8,
     )
     return out
 
@@ -217,11 +218,11 @@ def attn_tree(
         return out
     rows = N * (H // KVH)
     ctx = T if max_ctx is None else max(1, min(int(max_ctx), T))
-    wr, split = _plan(rows, B, B * rows, ctx, KVH, D)
+    wr, split, chunk = _plan(rows, lambda bm: B * -(-rows // bm), ctx, KVH, D, k_cache.dtype is _FP8)
     part, po, pm = _parts(split, B * N * H, D, q)
     _launch(
         _core.attn_tree, dev, q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-        p_slots, p_ctx, p_parents, out.data_ptr(), po, pm, strides, B, N, H, KVH, S, T, D, split, wr, scale,
+        p_slots, p_ctx, p_parents, out.data_ptr(), po, pm, strides, B, N, H, KVH, S, T, D, split, chunk, wr, scale,
         k_cache.dtype is _FP8,
     )
     return out
@@ -257,7 +258,7 @@ def tree_commit(
         raise ValueError(f"head dim must be a multiple of 8, got {D}")
     if N > MAX_NODES or (N < 1 and B > 0):
         raise ValueError(f"1 to {MAX_NODES} drafted nodes, got {N}")
-    strides = _rows("kv_new", kv_new) + _rows("kv_cache", kv_cache)
+    strides = _rows("kv_new", kv_new) + _rows("kv_cache", kv_cache, 16 if kv_cache.dtype is _BF16 else 8)
     given = (
         _index("slots", slots, (B,), dev), _index("ctx_lens", ctx_lens, (B,), dev),
         _index("parents", parents, (B, N), dev), _index("tokens", tokens, (B, N), dev, _I64),
