@@ -61,18 +61,9 @@ struct AttnArgs {
     long long k_ss, k_sh, k_st, v_ss, v_sh, v_st;
     long long kn_sb, kn_st, kn_sh, vn_sb, vn_st, vn_sh;
     int B, N, H, KVH, S, T;
-    int n_split, chunk;          // most splits of a row's keys, and tiles of one
+    int n_split;                 // most runs that a row's keys are split into
+    int share;                   // workgroups that the card takes at once, for each kv head
     float scale;
-};
-
-// How a tile of rows shares its key tiles out: runs of `per`, so that long rows have
-// many and short ones one, which writes its result itself.
-struct Runs {
-    int tiles, per, n;
-    __device__ __forceinline__ Runs(const AttnArgs& a, int tiles) : tiles(tiles) {
-        per = max(a.chunk, (tiles + a.n_split - 1) / a.n_split);
-        n = (tiles + per - 1) / per;
-    }
 };
 
 __device__ __forceinline__ int context(const AttnArgs& a, int b, bool tree) {
@@ -81,6 +72,51 @@ __device__ __forceinline__ int context(const AttnArgs& a, int b, bool tree) {
 // cache rows that the query rows up to `last_row` of a sequence see
 __device__ __forceinline__ int keys_of(const AttnArgs& a, int ctx, int last_row, int G, bool tree) {
     return tree ? ctx : max(0, min(ctx + last_row / G + 1, a.T));
+}
+
+// Where a sequence's rows lie, its tiles of rows, and the key tiles of the last of them
+// (0 tiles of rows for a padding entry whose keys are split: it is left to run 0).
+struct Seq {
+    int base, rows, row_tiles, key_tiles;
+    __device__ __forceinline__ Seq(const AttnArgs& a, int b, int G, int BM, int BN, bool tree) {
+        base = 0;
+        int len = a.N;
+        if (!tree) {
+            base = min(max(a.cu[b], 0), a.N);
+            len = min(max(a.cu[b + 1], base), a.N) - base;
+        }
+        rows = len * G;
+        row_tiles = (rows + BM - 1) / BM;
+        const int slot = a.slots[b];
+        key_tiles = 0;
+        if (slot >= 0 && slot < a.S && rows)
+            key_tiles = (keys_of(a, context(a, b, tree), rows - 1, G, tree) + BN - 1) / BN + (tree ? (a.N + BN - 1) / BN : 0);
+    }
+};
+
+// The keys of a tile of rows are split into runs of tiles, which workgroups take side by
+// side.  A run is as long as the tiles of all rows over the workgroups that the card
+// takes at once (less one for each tile of rows, whose last run is a part): then long
+// sequences have many runs and short ones one, which writes its result itself.  Every
+// wave of both kernels computes the same.
+__device__ __forceinline__ int run_length(const AttnArgs& a, int BM, int BN, bool tree) {
+    if (a.n_split == 1) return 0x7fffffff;
+    const int lane = threadIdx.x & 63, G = a.H / a.KVH;
+    float tiles = 0.f, rows = 0.f;
+    for (int b = lane; b < a.B; b += WAVE) {
+        const Seq s(a, b, G, BM, BN, tree);
+        tiles += (float)s.row_tiles * (float)s.key_tiles;
+        rows += (float)s.row_tiles;
+    }
+#pragma unroll
+    for (int o = 1; o < WAVE; o <<= 1) tiles += __shfl_xor(tiles, o, WAVE), rows += __shfl_xor(rows, o, WAVE);
+    const int per = (int)ceilf(tiles / fmaxf(1.f, (float)a.share - rows));
+    return __builtin_amdgcn_readfirstlane(max(per, 256 / BN));
+}
+
+// tiles of a run in a sequence whose last tile of rows has `most` key tiles
+__device__ __forceinline__ int run_of(const AttnArgs& a, int most, int length) {
+    return max(1, max(min(length, most), (most + a.n_split - 1) / a.n_split));
 }
 
 // max and sum over the two halves of a wave (lane and lane ^ 32)
@@ -271,6 +307,7 @@ struct Shape {
     static constexpr int RAW = TILE / 2;           // the same in 8 bits
     static constexpr int RAWS = 3;
     static constexpr int CHUNKS = 2 * TILE + (KV8 ? RAWS * RAW + (TREE ? TILE : 0) : 0);
+    static constexpr int SLOTS = KV8 || WR == 1 ? 256 : 512;  // workgroups that the card takes at once
     static constexpr int WAVES_A_SIMD = KV8 && WR == 2 ? 1 : WR == 1 ? 1 : 2;
 };
 
@@ -287,43 +324,44 @@ __global__ void __launch_bounds__((Shape<TREE, KV8, D, WR>::THREADS), (Shape<TRE
     const int half = lane >> 5, col = lane & 31;
     const int G = a.H / a.KVH;
     const int kvh = blockIdx.x % a.KVH;
-    const int split = blockIdx.y;
 
-    // which sequence and rows: tiles of ceil(len * G / BM) a sequence
-    int b, row0, rows, base;  // base: first token of the sequence in q
-    if constexpr (TREE) {
-        const int per = (a.N * G + BM - 1) / BM;
-        const int tile = blockIdx.x / a.KVH;
+    // Which sequence, rows and run: sequence b has ceil(rows / BM) tiles of rows, with
+    // as many runs each as its last one has.
+    const int length = run_length(a, BM, BN, TREE);
+    int b = -1, row0 = 0, rows = a.N * G, base = 0, split = 0;
+    if (TREE && a.n_split == 1) {
+        const int per = (rows + BM - 1) / BM, tile = blockIdx.x / a.KVH;
         b = tile / per;
-        row0 = (tile % per) * BM;
-        rows = a.N * G;
-        base = 0;
+        row0 = tile % per * BM;
     } else {
-        // the last tiles first: they see the most keys
-        int tile = gridDim.x / a.KVH - 1 - blockIdx.x / a.KVH;
-        b = -1;
-        row0 = rows = base = 0;
+        // the last ones first: they see the most keys
+        const int unit = gridDim.x / a.KVH - 1 - blockIdx.x / a.KVH;
         int before = 0;
         for (int b0 = 0; b0 < a.B; b0 += WAVE) {
-            int lo = 0, hi = 0;
+            int n = 0, runs = 1, first = 0, all = 0;
             if (b0 + lane < a.B) {
-                lo = min(max(a.cu[b0 + lane], 0), a.N);
-                hi = min(max(a.cu[b0 + lane + 1], lo), a.N);
+                const Seq s(a, b0 + lane, G, BM, BN, TREE);
+                first = s.base, all = s.rows;
+                const int per = run_of(a, s.key_tiles, length);
+                runs = max(1, (s.key_tiles + per - 1) / per);
+                n = s.row_tiles * runs;
             }
-            const int n = (int)(((long long)(hi - lo) * G + BM - 1) / BM);
             int sum = n;
 #pragma unroll
             for (int o = 1; o < WAVE; o <<= 1) {
                 const int up = __shfl_up(sum, o, WAVE);
                 if (lane >= o) sum += up;
             }
-            const unsigned long long found = __ballot(before + sum > tile);
+            const unsigned long long found = __ballot(before + sum > unit);
             if (found) {
                 const int l = __ffsll((long long)found) - 1;
                 b = b0 + l;
-                base = __builtin_amdgcn_readlane(lo, l);
-                rows = (__builtin_amdgcn_readlane(hi, l) - base) * G;
-                row0 = (tile - before - __builtin_amdgcn_readlane(sum - n, l)) * BM;
+                base = __builtin_amdgcn_readlane(first, l);
+                rows = __builtin_amdgcn_readlane(all, l);
+                const int i = unit - before - __builtin_amdgcn_readlane(sum - n, l);
+                runs = __builtin_amdgcn_readlane(runs, l);
+                row0 = i / runs * BM;
+                split = i % runs;
                 break;
             }
             before += __builtin_amdgcn_readlane(sum, WAVE - 1);
@@ -339,9 +377,12 @@ __global__ void __launch_bounds__((Shape<TREE, KV8, D, WR>::THREADS), (Shape<TRE
     const int kend = cached ? keys_of(a, ctx, last_row, G, TREE) : 0;
     const int ctx_tiles = (kend + BN - 1) / BN;
     const int new_tiles = TREE ? (a.N + BN - 1) / BN : 0;
-    const Runs runs(a, cached ? ctx_tiles + new_tiles : 0);
-    if (split > 0 && split >= runs.n) return;
-    const int t0 = split * runs.per, t1 = min(runs.tiles, t0 + runs.per);
+    const int tiles = cached ? ctx_tiles + new_tiles : 0;
+    const int most = cached ? (keys_of(a, ctx, rows - 1, G, TREE) + BN - 1) / BN + new_tiles : 0;
+    const int per = run_of(a, most, length);
+    const int runs = (tiles + per - 1) / per;
+    if (split > 0 && split >= runs) return;
+    const int t0 = split * per, t1 = min(tiles, t0 + per);
 
     // this lane's query row, and the last cache row that it sees
     const int row = row0 + wr * 32 + col;
@@ -568,7 +609,7 @@ __global__ void __launch_bounds__((Shape<TREE, KV8, D, WR>::THREADS), (Shape<TRE
     }
     if (!live) return;
     const int hb0 = WK > 1 ? wk * HW : 0;
-    if (runs.n > 1) {
+    if (runs > 1) {
         const size_t all_rows = (size_t)(TREE ? a.B * (long long)a.N : a.N);
         const size_t at = ((size_t)split * all_rows + (TREE ? (size_t)b * a.N : base) + token) * a.H + head;
 #pragma unroll
@@ -599,13 +640,13 @@ __global__ void __launch_bounds__((Shape<TREE, KV8, D, WR>::THREADS), (Shape<TRE
 
 // Joins the runs of a row that has several:
 //   out = sum_s 2^((m_s - m) c) O_s / sum_s 2^((m_s - m) c) l_s.
-// A workgroup has a (token, head), and each of its four waves every fourth load, which
-// covers 4 * 64 / D runs: all of a row's loads are on their way at once.
+// A wave has a (token, head); a load covers 256 / D runs, and up to 16 are on their way.
 template <bool TREE, int D>
 __global__ void __launch_bounds__(256) smg_attn_join_t(AttnArgs a, int BM, int BN) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63;
     const long long all_rows = TREE ? a.B * (long long)a.N : a.N;
-    const long long rh = blockIdx.x;
+    const long long rh = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (rh >= all_rows * a.H) return;
     const long long r = rh / a.H;
     const int h = (int)(rh % a.H), G = a.H / a.KVH;
     int b, rows, token;
@@ -632,22 +673,18 @@ __global__ void __launch_bounds__(256) smg_attn_join_t(AttnArgs a, int BM, int B
     const int slot = a.slots[b];
     if (slot < 0 || slot >= a.S) return;
     const int last_row = min((token * G + h % G) / BM * BM + BM, rows) - 1;
-    const int kend = keys_of(a, context(a, b, TREE), last_row, G, TREE);
-    const int n = Runs(a, (kend + BN - 1) / BN + (TREE ? (a.N + BN - 1) / BN : 0)).n;
+    const int ctx = context(a, b, TREE);
+    const int kend = keys_of(a, ctx, last_row, G, TREE);
+    const int new_tiles = TREE ? (a.N + BN - 1) / BN : 0;
+    const int most = (keys_of(a, ctx, rows - 1, G, TREE) + BN - 1) / BN + new_tiles;
+    const int per = run_of(a, most, run_length(a, BM, BN, TREE));
+    const int n = ((kend + BN - 1) / BN + new_tiles + per - 1) / per;
     if (n <= 1) return;
     // a lane a run (at most 64 of them)
     const float c = a.scale * LOG2E;
     const size_t run = all_rows * a.H;
     float ms = -INFINITY, ls = 0.f;
     if (lane < n) ms = a.part_ml[(lane * run + rh) * 2], ls = a.part_ml[(lane * run + rh) * 2 + 1];
-    constexpr int LPR = D / 4, RPL = WAVE / LPR;  // lanes of a row, rows of a load
-    const int e = lane % LPR * 4;
-    f32x4 part[WAVE / 4 / RPL];
-#pragma unroll
-    for (int i = 0; i < WAVE / 4 / RPL; ++i) {
-        const int s = (i * 4 + wave) * RPL + lane / LPR;
-        part[i] = s < n ? *(const f32x4*)(a.part_o + (s * run + rh) * D + e) : (f32x4)0.f;
-    }
     float top = ms;
 #pragma unroll
     for (int o = 1; o < WAVE; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, WAVE));
@@ -655,16 +692,24 @@ __global__ void __launch_bounds__(256) smg_attn_join_t(AttnArgs a, int BM, int B
     float sum = fs * ls;
 #pragma unroll
     for (int o = 1; o < WAVE; o <<= 1) sum += __shfl_xor(sum, o, WAVE);
+    constexpr int LPR = D / 4, RPL = WAVE / LPR;  // lanes of a row, rows of a load
+    const int e = lane % LPR * 4;
     f32x4 o = 0.f;
+    for (int s0 = 0; s0 < n; s0 += 16 * RPL) {
+        f32x4 part[16];
 #pragma unroll
-    for (int i = 0; i < WAVE / 4 / RPL; ++i) o += __shfl(fs, (i * 4 + wave) * RPL + lane / LPR, WAVE) * part[i];
-    __shared__ f32x4 rest[4][WAVE];
-    rest[wave][lane] = o;
-    __syncthreads();
-    if (threadIdx.x >= LPR) return;
-    o = 0.f;
+        for (int i = 0; i < 16; ++i) {
+            const int s = s0 + i * RPL + lane / LPR;
+            part[i] = s < n ? *(const f32x4*)(a.part_o + (s * run + rh) * D + e) : (f32x4)0.f;
+        }
 #pragma unroll
-    for (int i = 0; i < 4 * RPL; ++i) o += rest[i / RPL][i % RPL * LPR + lane];
+        for (int i = 0; i < 16; ++i) o += __shfl(fs, s0 + i * RPL + lane / LPR, WAVE) * part[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int step = LPR; step < WAVE; step <<= 1) o[i] += __shfl_xor(o[i], step, WAVE);
+    if (lane >= LPR) return;
     const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
     __hip_bfloat16* op = (TREE ? a.out + b * a.o_sb + token * a.o_st : a.out + r * a.o_st) + h * a.o_sh + e;
     bf16x4 w;
@@ -674,7 +719,7 @@ __global__ void __launch_bounds__(256) smg_attn_join_t(AttnArgs a, int BM, int B
 }
 
 template <bool TREE, bool KV8, int D, int WR>
-int launch_t(AttnArgs a, int chunk_keys, hipStream_t s) {
+int launch_t(AttnArgs a, hipStream_t s) {
     using Z = Shape<TREE, KV8, D, WR>;
     constexpr int BM = Z::BM, BN = Z::BN;
     constexpr int tile_bytes = Z::CHUNKS * 16;
@@ -683,8 +728,9 @@ int launch_t(AttnArgs a, int chunk_keys, hipStream_t s) {
     static_assert(bytes <= 160 * 1024, "LDS of a compute unit");
     const long long G = a.H / a.KVH;
     const long long tiles = TREE ? a.B * ((a.N * G + BM - 1) / BM) : a.N * G / BM + a.B;
-    const long long grid = tiles * a.KVH;
-    a.chunk = (chunk_keys + BN - 1) / BN;
+    // with runs: never more than `share` of them, but at least one for each tile of rows
+    a.share = (int)(Z::SLOTS / a.KVH > tiles ? Z::SLOTS / a.KVH : tiles);
+    const long long grid = (a.n_split > 1 ? a.share : tiles) * a.KVH;
     if (grid > 0x7fffffffll || a.n_split > WAVE) return -5;
     // more dynamic LDS than the default limit, once a device
     static std::atomic<unsigned long long> set{0};
@@ -696,32 +742,32 @@ int launch_t(AttnArgs a, int chunk_keys, hipStream_t s) {
             return -2;
         if (dev <= 63) set.fetch_or(1ull << dev, std::memory_order_relaxed);
     }
-    hipLaunchKernelGGL((smg_attn_cache_t<TREE, KV8, D, WR>), dim3((unsigned)grid, a.n_split), dim3(Z::THREADS), bytes, s, a);
+    hipLaunchKernelGGL((smg_attn_cache_t<TREE, KV8, D, WR>), dim3((unsigned)grid), dim3(Z::THREADS), bytes, s, a);
     if (a.n_split > 1) {
         const long long rh = (TREE ? a.B * (long long)a.N : a.N) * a.H;
         if (rh > 0x7fffffffll) return -5;
-        hipLaunchKernelGGL((smg_attn_join_t<TREE, D>), dim3((unsigned)rh), dim3(256), 0, s, a, BM, BN);
+        hipLaunchKernelGGL((smg_attn_join_t<TREE, D>), dim3((unsigned)((rh + 3) / 4)), dim3(256), 0, s, a, BM, BN);
     }
     return hipGetLastError() == hipSuccess ? 0 : -2;
 }
 
 template <bool TREE, bool KV8, int D>
-int launch_d(const AttnArgs& a, int wr, int chunk, hipStream_t s) {
+int launch_d(const AttnArgs& a, int wr, hipStream_t s) {
     if constexpr (KV8) {
-        if (wr <= 2) return launch_t<TREE, true, D, 2>(a, chunk, s);
-        if (wr == 4) return launch_t<TREE, true, D, 4>(a, chunk, s);
-        return launch_t<TREE, true, D, 8>(a, chunk, s);
+        if (wr <= 2) return launch_t<TREE, true, D, 2>(a, s);
+        if (wr == 4) return launch_t<TREE, true, D, 4>(a, s);
+        return launch_t<TREE, true, D, 8>(a, s);
     } else {
         if constexpr (D == 128)
-            if (wr == 1) return launch_t<TREE, false, D, 1>(a, chunk, s);
-        if (wr <= 2) return launch_t<TREE, false, D, 2>(a, chunk, s);
-        return launch_t<TREE, false, D, 4>(a, chunk, s);
+            if (wr == 1) return launch_t<TREE, false, D, 1>(a, s);
+        if (wr <= 2) return launch_t<TREE, false, D, 2>(a, s);
+        return launch_t<TREE, false, D, 4>(a, s);
     }
 }
 
 template <bool TREE, bool KV8>
-int launch(const AttnArgs& a, int D, int wr, int chunk, hipStream_t s) {
-    return D == 128 ? launch_d<TREE, KV8, 128>(a, wr, chunk, s) : D == 64 ? launch_d<TREE, KV8, 64>(a, wr, chunk, s) : -1;
+int launch(const AttnArgs& a, int D, int wr, hipStream_t s) {
+    return D == 128 ? launch_d<TREE, KV8, 128>(a, wr, s) : D == 64 ? launch_d<TREE, KV8, 64>(a, wr, s) : -1;
 }
 
 int bad_shape(int H, int KVH, int S, int T, int n_split) {
@@ -736,9 +782,8 @@ int bad_shape(int H, int KVH, int S, int T, int n_split) {
 extern "C" int smg_attn_prefill_launch(
     const void* q, const void* k, const void* v, const void* slots, const void* ctx, const void* cu,
     void* out, void* part_o, void* part_ml, const long long* strides, int B, int N, int H, int KVH,
-    int S, int T, int D, int n_split, int chunk, int wr, float scale, int kv_fp8, void* stream) {
+    int S, int T, int D, int n_split, int wr, float scale, int kv_fp8, void* stream) {
     if (int rc = bad_shape(H, KVH, S, T, n_split)) return rc;
-    if (chunk < 1) return -3;
     if (B < 1 || N < 1) return 0;
     AttnArgs a = {};
     a.q = (const __hip_bfloat16*)q;
@@ -755,18 +800,17 @@ extern "C" int smg_attn_prefill_launch(
     a.v_ss = strides[7], a.v_sh = strides[8], a.v_st = strides[9];
     a.B = B, a.N = N, a.H = H, a.KVH = KVH, a.S = S, a.T = T, a.n_split = n_split;
     a.scale = scale;
-    return kv_fp8 ? launch<false, true>(a, D, wr, chunk, (hipStream_t)stream)
-                  : launch<false, false>(a, D, wr, chunk, (hipStream_t)stream);
+    return kv_fp8 ? launch<false, true>(a, D, wr, (hipStream_t)stream)
+                  : launch<false, false>(a, D, wr, (hipStream_t)stream);
 }
 
 // strides: q batch/token/head, out batch/token/head, k and v as above, k_new and v_new batch/token/head
 extern "C" int smg_attn_tree_launch(
     const void* q, const void* k_new, const void* v_new, const void* k, const void* v,
     const void* slots, const void* ctx, const void* parents, void* out, void* part_o, void* part_ml,
-    const long long* strides, int B, int N, int H, int KVH, int S, int T, int D, int n_split,
-    int chunk, int wr, float scale, int kv_fp8, void* stream) {
+    const long long* strides, int B, int N, int H, int KVH, int S, int T, int D, int n_split, int wr,
+    float scale, int kv_fp8, void* stream) {
     if (int rc = bad_shape(H, KVH, S, T, n_split)) return rc;
-    if (chunk < 1) return -3;
     if (N > 64) return -3;
     if (B < 1 || N < 1) return 0;
     AttnArgs a = {};
@@ -789,6 +833,6 @@ extern "C" int smg_attn_tree_launch(
     a.vn_sb = strides[15], a.vn_st = strides[16], a.vn_sh = strides[17];
     a.B = B, a.N = N, a.H = H, a.KVH = KVH, a.S = S, a.T = T, a.n_split = n_split;
     a.scale = scale;
-    return kv_fp8 ? launch<true, true>(a, D, wr, chunk, (hipStream_t)stream)
-                  : launch<true, false>(a, D, wr, chunk, (hipStream_t)stream);
+    return kv_fp8 ? launch<true, true>(a, D, wr, (hipStream_t)stream)
+                  : launch<true, false>(a, D, wr, (hipStream_t)stream);
 }

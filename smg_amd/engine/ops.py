@@ -119,17 +119,18 @@ def _launch(kernel, dev: int, *args) -> None:
             kernel(*args, stream)
 
 
-_WORK = 512  # workgroups that fill the card, where rows alone give fewer
+_SPLIT_BELOW = 256  # workgroups by rows alone, above which keys are not split
 
 
-def _plan(rows: int, tiles, ctx: int, KVH: int, D: int, fp8: bool) -> Tuple[int, int, int]:
-    """(waves along the query rows, most splits of the keys, keys of a split) for
-    sequences of about `rows` rows a kv head and up to `ctx` keys; tiles(rows of a
-    tile) is how many tiles of rows there are."""
+def _plan(rows: int, tiles, ctx: int, KVH: int, D: int, fp8: bool) -> Tuple[int, int]:
+    """(waves along the query rows, most runs of a row's keys) for sequences of about
+    `rows` rows a kv head and up to `ctx` keys; tiles(rows of a tile) is how many
+    tiles of rows there are.  The kernel sizes the runs by the sequences' lengths."""
     wr = 1 if rows <= 32 and D == 128 and not fp8 else 2 if rows <= 64 else 8 if fp8 and rows > 128 else 4
     work = tiles(32 * wr) * KVH
-    split = 1 if work >= 256 else max(1, min(_WORK // work, ctx // 256, 64))
-    return wr, split, -(-ctx // split)
+    if work >= _SPLIT_BELOW:
+        return wr, 1
+    return wr, max(1, min(64, ctx // 256))
 
 
 def _parts(split: int, rows: int, D: int, q: torch.Tensor) -> tuple:
@@ -172,11 +173,11 @@ def attn_prefill(
         return out
     total = N * (H // KVH)
     ctx = T if max_ctx is None else max(1, min(int(max_ctx), T))
-    wr, split, chunk = _plan(total // B, lambda bm: total // bm + B, ctx, KVH, D, k_cache.dtype is _FP8)
+    wr, split = _plan(total // B, lambda bm: total // bm + B, ctx, KVH, D, k_cache.dtype is _FP8)
     part, po, pm = _parts(split, N * H, D, q)
     _launch(
         _core.attn_prefill, dev, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), p_slots, p_starts, p_cu,
-        out.data_ptr(), po, pm, strides, B, N, H, KVH, S, T, D, split, chunk, wr, scale, k_cache.dtype is _FP8,
+        out.data_ptr(), po, pm, strides, B, N, H, KVH, S, T, D, split, wr, scale, k_cache.dtype is _FP8,
     )
     return out
 
@@ -218,11 +219,11 @@ def attn_tree(
         return out
     rows = N * (H // KVH)
     ctx = T if max_ctx is None else max(1, min(int(max_ctx), T))
-    wr, split, chunk = _plan(rows, lambda bm: B * -(-rows // bm), ctx, KVH, D, k_cache.dtype is _FP8)
+    wr, split = _plan(rows, lambda bm: B * -(-rows // bm), ctx, KVH, D, k_cache.dtype is _FP8)
     part, po, pm = _parts(split, B * N * H, D, q)
     _launch(
         _core.attn_tree, dev, q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-        p_slots, p_ctx, p_parents, out.data_ptr(), po, pm, strides, B, N, H, KVH, S, T, D, split, chunk, wr, scale,
+        p_slots, p_ctx, p_parents, out.data_ptr(), po, pm, strides, B, N, H, KVH, S, T, D, split, wr, scale,
         k_cache.dtype is _FP8,
     )
     return out
