@@ -48,17 +48,16 @@ def _check(name: str, t, dtypes: tuple, dim: int, dev: Optional[int]) -> None:
 def _rows(name: str, t: torch.Tensor, unit: int = 16) -> tuple:
     """The strides but the last, of a tensor that is dense in its last dimension and
     whose rows start at multiples of `unit` bytes."""
-    strides = t.stride()
-    e = t.element_size()
-    at = t.data_ptr()
-    for s in strides[:-1]:
+    *strides, last = t.stride()
+    at, e = t.data_ptr(), t.element_size()
+    for s in strides:
         at |= s * e
-    if (strides[-1] != 1 or at % unit) and t.numel():
-        if strides[-1] != 1:
-            raise ValueError(f"{name} must be dense in its last dimension, strides {strides}")
-        if t.data_ptr() % unit or any(s * e % unit for s, n in zip(strides[:-1], t.shape) if n > 1):
-            raise ValueError(f"{name}: rows must start at multiples of {unit} bytes, strides {strides}")
-    return strides[:-1]
+    if (last != 1 or at % unit) and t.numel():
+        if last != 1:
+            raise ValueError(f"{name} must be dense in its last dimension, strides {t.stride()}")
+        if t.data_ptr() % unit or any(s * e % unit for s, n in zip(strides, t.shape) if n > 1):
+            raise ValueError(f"{name}: rows must start at multiples of {unit} bytes, strides {t.stride()}")
+    return strides
 
 
 def _index(name: str, t, shape: tuple, dev: int, dtype: torch.dtype = _I32) -> int:
@@ -73,13 +72,12 @@ def _cache(k: torch.Tensor, v: torch.Tensor, dev: int, H: int, D: int) -> tuple:
     """(slots, kv heads, positions) and the strides of both."""
     _check("k_cache", k, _CACHE_TYPES, 4, dev)
     _check("v_cache", v, _CACHE_TYPES, 4, dev)
-    shape = k.shape
+    S, KVH, T, d = shape = k.shape
     if shape != v.shape or k.dtype is not v.dtype:
         raise ValueError(f"k_cache {tuple(shape)} {k.dtype} and v_cache {tuple(v.shape)} {v.dtype} differ")
-    S, KVH, T, d = shape
     if d != D or D not in HEAD_DIMS:
         raise ValueError(f"head dim must be one of {HEAD_DIMS} and equal, got {D} over a cache of {d}")
-    if min(S, KVH, T) < 1 or H < 1 or H % KVH:
+    if S < 1 or KVH < 1 or T < 1 or H < 1 or H % KVH:
         raise ValueError(f"{H} heads over a cache of {tuple(shape)}")
     return S, KVH, T, _rows("k_cache", k) + _rows("v_cache", v)
 
@@ -95,7 +93,7 @@ def _scale(scale: Optional[float], D: int) -> float:
 
 def _out(out: Optional[torch.Tensor], q: torch.Tensor, dev: int) -> torch.Tensor:
     if out is None:
-        return q.new_empty(q.shape)
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
     _check("out", out, (_BF16,), q.dim(), dev)
     if out.shape != q.shape:
         raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
@@ -122,15 +120,18 @@ def _launch(kernel, dev: int, *args) -> None:
 _SPLIT_BELOW = 256  # workgroups by rows alone, above which keys are not split
 
 
-def _plan(rows: int, tiles, ctx: int, KVH: int, D: int, fp8: bool) -> Tuple[int, int]:
-    """(waves along the query rows, most runs of a row's keys) for sequences of about
-    `rows` rows a kv head and up to `ctx` keys; tiles(rows of a tile) is how many
-    tiles of rows there are.  The kernel sizes the runs by the sequences' lengths."""
-    wr = 1 if rows <= 32 and D == 128 and not fp8 else 2 if rows <= 64 else 8 if fp8 and rows > 128 else 4
-    work = tiles(32 * wr) * KVH
-    if work >= _SPLIT_BELOW:
-        return wr, 1
-    return wr, max(1, min(64, ctx // 256))
+def _waves(rows: int, D: int, fp8: bool) -> int:
+    """Waves along the query rows (32 each) of a workgroup, for sequences of about
+    `rows` rows a kv head."""
+    if rows <= 64:
+        return 1 if rows <= 32 and D == 128 and not fp8 else 2
+    return 8 if fp8 and rows > 128 else 4
+
+
+def _splits(work: int, ctx: int) -> int:
+    """Most runs of a row's keys, where the rows alone give `work` workgroups.  The
+    kernel sizes the runs by the sequences' lengths."""
+    return 1 if work >= _SPLIT_BELOW else max(1, min(64, ctx // 256))
 
 
 def _parts(split: int, rows: int, D: int, q: torch.Tensor) -> tuple:
@@ -172,12 +173,13 @@ def attn_prefill(
     if N == 0 or B == 0:
         return out
     total = N * (H // KVH)
-    ctx = T if max_ctx is None else max(1, min(int(max_ctx), T))
-    wr, split = _plan(total // B, lambda bm: total // bm + B, ctx, KVH, D, k_cache.dtype is _FP8)
+    fp8 = k_cache.dtype is _FP8
+    wr = _waves(total // B, D, fp8)
+    split = _splits((total // (32 * wr) + B) * KVH, T if max_ctx is None else min(int(max_ctx), T))
     part, po, pm = _parts(split, N * H, D, q)
     _launch(
         _core.attn_prefill, dev, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), p_slots, p_starts, p_cu,
-        out.data_ptr(), po, pm, strides, B, N, H, KVH, S, T, D, split, wr, scale, k_cache.dtype is _FP8,
+        out.data_ptr(), po, pm, strides, B, N, H, KVH, S, T, D, split, wr, scale, fp8,
     )
     return out
 
@@ -218,13 +220,13 @@ def attn_tree(
     if B == 0 or N == 0:
         return out
     rows = N * (H // KVH)
-    ctx = T if max_ctx is None else max(1, min(int(max_ctx), T))
-    wr, split = _plan(rows, lambda bm: B * -(-rows // bm), ctx, KVH, D, k_cache.dtype is _FP8)
+    fp8 = k_cache.dtype is _FP8
+    wr = _waves(rows, D, fp8)
+    split = _splits(B * -(-rows // (32 * wr)) * KVH, T if max_ctx is None else min(int(max_ctx), T))
     part, po, pm = _parts(split, B * N * H, D, q)
     _launch(
         _core.attn_tree, dev, q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-        p_slots, p_ctx, p_parents, out.data_ptr(), po, pm, strides, B, N, H, KVH, S, T, D, split, wr, scale,
-        k_cache.dtype is _FP8,
+        p_slots, p_ctx, p_parents, out.data_ptr(), po, pm, strides, B, N, H, KVH, S, T, D, split, wr, scale, fp8,
     )
     return out
 
@@ -266,7 +268,7 @@ def tree_commit(
         _index("targets", targets, (B, N), dev, _I64),
     )
     _on_gpu("kv_new", kv_new, dev)
-    count, path, nxt = ctx_lens.new_empty(B), parents.new_empty((B, N)), tokens.new_empty(B)
+    count, path, nxt = torch.empty_like(ctx_lens), torch.empty_like(parents), tokens.new_empty(B)
     if B:
         _launch(
             _core.tree_commit, dev, kv_new.data_ptr(), kv_cache.data_ptr(), *given, count.data_ptr(), path.data_ptr(),
