@@ -96,7 +96,8 @@ int smg_tree_commit_launch(const void* src, void* dst, const void* slots, const 
 // ---- sampling (sample.hip) ----
 int smg_sample_launch(const void* logits, const void* u, const void* temperature,
                       const void* top_k, const void* top_p, const void* min_p, void* out,
-                      long long stride, int R, int V, int f32, void* stream);
+                      void* work, long long stride, int R, int V, int parts, int f32, void* stream);
+long long smg_sample_work_bytes();
 // ---- fused decode elementwise (fused_decode.hip) ----
 int smg_rope_kv_store_launch(const void* qkv, const void* freqs, const void* pos,
                              void* k_cache, void* v_cache, void* q_out,
@@ -564,17 +565,18 @@ PYBIND11_MODULE(_core, m) {
     // temperature / top-k / top-p / min-p sampling (sample.hip)
     m.def("sample",
           [](uintptr_t logits, uintptr_t u, uintptr_t temperature, uintptr_t top_k, uintptr_t top_p,
-             uintptr_t min_p, uintptr_t out, long long stride, int R, int V, int f32,
-             uintptr_t stream) {
+             uintptr_t min_p, uintptr_t out, uintptr_t work, long long stride, int R, int V,
+             int parts, int f32, uintptr_t stream) {
               int rc = smg_sample_launch((const void*)logits, (const void*)u,
                                          (const void*)temperature, (const void*)top_k,
-                                         (const void*)top_p, (const void*)min_p, (void*)out, stride,
-                                         R, V, f32, (void*)stream);
+                                         (const void*)top_p, (const void*)min_p, (void*)out,
+                                         (void*)work, stride, R, V, parts, f32, (void*)stream);
               if (rc != 0) throw std::runtime_error("sample launch failed rc=" + std::to_string(rc));
           },
           py::arg("logits"), py::arg("u"), py::arg("temperature"), py::arg("top_k"),
-          py::arg("top_p"), py::arg("min_p"), py::arg("out"), py::arg("stride"), py::arg("R"),
-          py::arg("V"), py::arg("f32"), py::arg("stream"));
+          py::arg("top_p"), py::arg("min_p"), py::arg("out"), py::arg("work"), py::arg("stride"),
+          py::arg("R"), py::arg("V"), py::arg("parts"), py::arg("f32"), py::arg("stream"));
+    m.def("sample_work_bytes", &smg_sample_work_bytes);
 
     py::class_<PyHostTree>(m, "HostTokenTree")
         .def(py::init<uint32_t>(), py::arg("page_size") = 16)

@@ -38,6 +38,8 @@
 #define BLOCK 512           // tokens of a wave's iteration
 #define CAND 128            // tokens that are compared with each other
 #define MAX_V (NB * BLOCK)
+#define DEEP 2              // loads of a wave on their way
+#define MAX_PARTS 16        // workgroups of a row
 
 namespace {
 
@@ -54,6 +56,20 @@ struct SampleArgs {
     const float* min_p;        // [R] or null
     long long* out;            // [R]
     int R, V;
+    u64* work;                 // split rows: [R] of Work
+    int parts;                 // workgroups that share a row (1: none do)
+};
+
+// What the workgroups of a row leave for each other.
+struct Work {
+    u64 hist[NB];        // of the first cut's measure
+    u64 blocks[NB];      // sums of weights, 512 tokens each
+    float lo[MAX_PARTS], hi[MAX_PARTS];
+    int first[MAX_PARTS];  // the first index of each part's largest
+    float x;             // what the cuts keep, if `open`
+    int i;
+    int open;            // whether the row still needs its answer
+    int pad;
 };
 
 struct Shared {
@@ -133,8 +149,15 @@ __device__ __forceinline__ T before_wave(const T* v, T* all) {
 
 __device__ __forceinline__ void clear(Shared& sh) {
     __syncthreads();
-    sh.hist[threadIdx.x] = sh.hist[threadIdx.x + THREADS] = 0;
+#pragma unroll
+    for (int i = 0; i < NB / THREADS; ++i) sh.hist[threadIdx.x + i * THREADS] = 0;
     __syncthreads();
+}
+
+__device__ __forceinline__ void load(Shared& sh, const u64* from, int n) {
+    __syncthreads();
+#pragma unroll
+    for (int i = threadIdx.x; i < NB; i += THREADS) sh.hist[i] = i < n ? from[i] : 0;
 }
 
 // Adds the NB counters of sh.hist up: sh.bin and sh.above get the first at which
@@ -142,20 +165,27 @@ __device__ __forceinline__ void clear(Shared& sh) {
 // does).  Returns that want.
 template <typename W>
 __device__ __forceinline__ u64 locate(Shared& sh, W&& want_of) {
+    constexpr int OWN = NB / THREADS;  // counters of a thread
     const int t = threadIdx.x;
     __syncthreads();
-    const u64 a = sh.hist[2 * t], s = a + sh.hist[2 * t + 1];
-    const u64 run = wave_scan(s);
+    u64 sum[OWN];
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) sum[i] = sh.hist[OWN * t + i] + (i ? sum[i - 1] : 0);
+    const u64 run = wave_scan(sum[OWN - 1]);
     if ((t & 63) == 63) sh.part[t / WAVE] = run;
     if (t == 0) sh.bin = NB;
     __syncthreads();
     u64 all;
-    const u64 before = before_wave(sh.part, &all) + run - s;
+    const u64 before = before_wave(sh.part, &all) + run - sum[OWN - 1];
     const u64 want = want_of(all);
-    if (before < want && before + s >= want) {
-        const bool second = before + a < want;
-        sh.bin = 2 * t + second;
-        sh.above = before + (second ? a : 0);
+    if (before < want && before + sum[OWN - 1] >= want) {
+        int n = 0;
+        u64 above = before;
+#pragma unroll
+        for (int i = 0; i < OWN - 1; ++i)
+            if (before + sum[i] < want) n = i + 1, above = before + sum[i];
+        sh.bin = OWN * t + n;
+        sh.above = above;
     }
     __syncthreads();
     return want;
@@ -212,8 +242,9 @@ struct Weigh {
 // FEW: V < 8, where 8 tokens cannot be loaded at once.
 template <bool F32, bool FEW>
 struct Row {
+    static constexpr bool LISTED = false;
     const char* at;
-    int V, start, its, lane;
+    int V, start, end, its, lane;  // this wave's run, in `its` iterations at most
 
     struct Raw {
         u32x4 w[F32 ? 2 : 1];
@@ -255,12 +286,15 @@ struct Row {
         }
         return r;
     }
-    __device__ __forceinline__ void init(const SampleArgs& a) {
+    // row r, or part `part` of `parts` of it
+    __device__ __forceinline__ void init(const SampleArgs& a, int r, int part = 0, int parts = 1) {
         lane = threadIdx.x & 63;
         V = a.V;
-        at = (const char*)a.logits + blockIdx.x * a.stride * (F32 ? 4 : 2);
-        its = (V + WAVES * BLOCK - 1) / (WAVES * BLOCK);
-        start = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE) * its * BLOCK;
+        at = (const char*)a.logits + r * a.stride * (F32 ? 4 : 2);
+        const int blocks = (V + BLOCK - 1) / BLOCK, mine = (blocks + parts - 1) / parts;
+        its = (mine + WAVES - 1) / WAVES;
+        end = min(V, (part + 1) * mine * BLOCK);
+        start = part * mine * BLOCK + __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE) * its * BLOCK;
     }
     template <typename F>
     __device__ __forceinline__ void each8(int it, const Raw& r, F&& f) const {
@@ -268,33 +302,56 @@ struct Row {
 #pragma unroll
         for (int e = 0; e < 8; ++e) f(b + e, r[e]);
     }
-    // g(it, raw) for each iteration that has tokens, the next one's on their way
+    // g(it, raw) for each iteration that has tokens: DEEP loads at once
     template <typename G>
     __device__ __forceinline__ void blocks(G&& g) const {
-        const int n = min(its, (V - start + BLOCK - 1) / BLOCK);
-        if (n <= 0) return;
-        Raw next = load8(0);
-        for (int it = 0; it < n; ++it) {
-            const Raw now = next;
-            if (it + 1 < n) next = load8(it + 1);
-            g(it, now);
+        const int n = min(its, (end - start + BLOCK - 1) / BLOCK);
+        for (int i0 = 0; i0 < n; i0 += DEEP) {
+            Raw r[DEEP];
+#pragma unroll
+            for (int i = 0; i < DEEP; ++i)
+                if (i0 + i < n) r[i] = load8(i0 + i);
+#pragma unroll
+            for (int i = 0; i < DEEP; ++i)
+                if (i0 + i < n) g(i0 + i, r[i]);
         }
     }
     template <typename F>
     __device__ __forceinline__ void each(F&& f) const {
         blocks([&](int it, const Raw& r) { each8(it, r, f); });
     }
-    // The first index at which the sums of measure(i, x), by index, reach
-    // want(sum of all), which is at least 1 and at most that.
-    template <typename W, typename M>
-    __device__ __forceinline__ int find(Shared& sh, W&& want_of, M&& measure) const {
-        clear(sh);
+    // f(x, measure(i, x)) where that is not 0; the measures of 8 tokens side by side
+    template <typename M, typename F>
+    __device__ __forceinline__ void weighed(M&& measure, F&& f) const {
+        blocks([&](int it, const Raw& r) {
+            u64 w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = measure(base(it) + e, r[e]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (w[e]) f(r[e], w[e]);
+        });
+    }
+    // Sums of measure(i, x) over 512 tokens each.
+    template <typename M>
+    __device__ __forceinline__ void sums(u64* to, M&& measure) const {
         blocks([&](int it, const Raw& r) {
             u64 s = 0;
             each8(it, r, [&](int i, float x) { s += measure(i, x); });
             s = wave_sum(s);
-            if (lane == 0) sh.hist[start / BLOCK + it] = s;
+            if (lane == 0) to[start / BLOCK + it] = s;
         });
+    }
+    // The first index at which the sums of measure(i, x), by index, reach
+    // want(sum of all), which is at least 1 and at most that.  `given`: those sums.
+    template <typename W, typename M>
+    __device__ __forceinline__ int find(Shared& sh, W&& want_of, M&& measure, const u64* given = nullptr) const {
+        if (given) {
+            load(sh, given, (V + BLOCK - 1) / BLOCK);
+        } else {
+            clear(sh);
+            sums(sh.hist, measure);
+        }
         u64 want = locate(sh, want_of);
         const int it = sh.bin - start / BLOCK;
         if (it >= 0 && it < its) {
@@ -343,24 +400,33 @@ struct Row {
     }
 };
 
-// The tokens that a cut left: i is their place in the list, two a thread.
+// The tokens that a cut left: i is their place in the list.
 struct List {
+    static constexpr bool LISTED = true;
+    static constexpr int OWN = NB / THREADS;  // tokens of a thread
     Shared* sh;
     int n;
     template <typename F>
     __device__ __forceinline__ void each(F&& f) const {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int i = 2 * threadIdx.x + e;
+        for (int e = 0; e < OWN; ++e) {
+            const int i = OWN * threadIdx.x + e;
             if (i < n) f(i, sh->list_x[i]);
         }
+    }
+    template <typename M, typename F>
+    __device__ __forceinline__ void weighed(M&& measure, F&& f) const {
+        each([&](int i, float x) {
+            const u64 w = measure(i, x);
+            if (w) f(x, w);
+        });
     }
     template <typename W, typename M>
     __device__ __forceinline__ int find(Shared& s, W&& want_of, M&& measure) const {
         __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int i = 2 * threadIdx.x + e;
+        for (int e = 0; e < OWN; ++e) {
+            const int i = OWN * threadIdx.x + e;
             s.hist[i] = i < n ? measure(i, s.list_x[i]) : 0;
         }
         locate(s, want_of);
@@ -383,19 +449,24 @@ struct Search {
         if (counting) return (u64)from.has(x, i);
         return weigh.fixed(x, from.has(x, i));
     }
-    // The step in which want(sum of all) is reached, NB - 1 or NB if it never is.
-    template <typename W>
-    __device__ __forceinline__ u64 divide(W&& want_of) const {
+    // The measure of each step, into sh.hist.
+    __device__ __forceinline__ void fill() const {
         clear(sh);
         if (counting)
             tokens.each([&](int i, float x) {
                 if (from.has(x, i)) atomicAdd(&sh.hist[step(x)], 1ull);
             });
         else
-            tokens.each([&](int i, float x) {
-                const u64 w = weigh.fixed(x, from.has(x, i));
-                if (w) atomicAdd(&sh.hist[step(x)], w);
-            });
+            tokens.weighed([&](int i, float x) { return weigh.fixed(x, from.has(x, i)); },
+                           [&](float x, u64 w) { atomicAdd(&sh.hist[step(x)], w); });
+    }
+    // The step in which want(sum of all) is reached, NB - 1 or NB if it never is.
+    template <typename W>
+    __device__ __forceinline__ u64 divide(W&& want_of, const u64* given = nullptr) const {
+        if (given)
+            load(sh, given, NB);
+        else
+            fill();
         return locate(sh, want_of);
     }
     // The prefix, from the step `bin` in which `want` is reached and the measure
@@ -422,7 +493,7 @@ struct Search {
             __syncthreads();
             const int n = sh.count;
             if (n <= CAND) {
-                // every eighth candidate, from this thread's first on, that comes before
+                // some of the candidates, from this thread's first on, that come before
                 // this thread's own
                 const int me = threadIdx.x & (CAND - 1), first = threadIdx.x / CAND;
                 const float x = sh.cand_x[me];
@@ -463,8 +534,8 @@ struct Search {
         }
     }
     template <typename W>
-    __device__ __forceinline__ Prefix operator()(W&& want_of) const {
-        const u64 want = divide(want_of);
+    __device__ __forceinline__ Prefix operator()(W&& want_of, const u64* given = nullptr) const {
+        const u64 want = divide(want_of, given);
         return sh.bin >= NB - 1 ? from : within(sh.bin, sh.above, want);
     }
 };
@@ -474,141 +545,307 @@ __device__ __forceinline__ u64 share(float p, u64 all) {  // the measure that to
     return want >= 1. ? (u64)want : 1;
 }
 
-// The first token by index at which the weights that `kept` and min-p leave reach
-// more than u of their sum.
-template <bool CUT, typename T>
-__device__ __forceinline__ int draw(Shared& sh, const T& tokens, const Weigh& weigh, Prefix kept, float u, float min_p) {
-    const double least = min_p > 0.f ? fmin((double)min_p, 1.) * weigh.units : 0.;
-    return tokens.find(
-        sh,
-        [&](u64 all) {
-            const double aim = u > 0.f ? (double)u * (double)all : 0.;
-            return aim < (double)all ? (u64)aim + 1 : all;
-        },
-        [&](int i, float x) {
-            const double w = weigh.scaled(x);
-            const bool live = (x >= weigh.floor) & (w >= least);
-            return (CUT ? live & kept.has(x, i) : live) ? weigh.rounded(w) : 0ull;
-        });
+struct Step {
+    float cap, per;
+    __device__ __forceinline__ int operator()(float x) const { return (int)fminf((cap - fminf(x, cap)) * per, NB - 1.f); }
+};
+
+// A row's settings, and what follows from its largest and smallest logit.
+struct Plan {
+    Weigh weigh;
+    Step step;
+    Prefix all;  // everything above -inf, or the +inf
+    int k;
+    float p, u, t;
+    double least;  // the smallest weight that min-p keeps, in units
+    bool by_count, by_mass;
+
+    __device__ __forceinline__ Plan(const SampleArgs& a, int r) {
+        t = a.temperature[r];
+        k = a.top_k ? a.top_k[r] : 0;
+        p = a.top_p ? a.top_p[r] : 1.f;
+        u = a.u[r];
+        by_count = k > 0 && k < a.V;
+        by_mass = p < 1.f;
+    }
+    __device__ __forceinline__ void init(Shared& sh, const SampleArgs& a, int r, float2 ends) {
+        weigh.init(sh, ends.y, t, a.V);
+        // steps down from the largest: to the smallest, or to where weights are 0
+        // (below 2^-51), whose tokens the last step takes
+        const float depth = fminf(weigh.cap - ends.x, 51.f * 0.69314718f * t);
+        step = {weigh.cap, depth > 1e-30f ? (NB - 2) / depth : 0.f};
+        all = {ends.y == INFINITY ? weigh.cap : -INFINITY, -1};
+        const float mp = a.min_p ? a.min_p[r] : 0.f;
+        least = mp > 0.f ? fmin((double)mp, 1.) * weigh.units : 0.;
+    }
+    // the weights that `kept` and min-p leave
+    template <bool CUT>
+    __device__ __forceinline__ u64 left(Prefix kept, int i, float x) const {
+        const double w = weigh.scaled(x);
+        const bool live = (x >= weigh.floor) & (w >= least);
+        return (CUT ? live & kept.has(x, i) : live) ? weigh.rounded(w) : 0ull;
+    }
+    // the first token by index at which they reach more than u of their sum
+    template <bool CUT, typename T>
+    __device__ __forceinline__ int draw(Shared& sh, const T& tokens, Prefix kept, const u64* given = nullptr) const {
+        auto want_of = [&](u64 sum) {
+            const double aim = u > 0.f ? (double)u * (double)sum : 0.;
+            return aim < (double)sum ? (u64)aim + 1 : sum;
+        };
+        auto measure = [&](int i, float x) { return left<CUT>(kept, i, x); };
+        if constexpr (T::LISTED)
+            return tokens.find(sh, want_of, measure);
+        else
+            return tokens.find(sh, want_of, measure, given);
+    }
+};
+
+// Top-k, then top-p: what they keep, as a prefix of the list if that holds it
+// (list.n <= NB), else of the row.  hi: the largest of this thread's tokens; given: the
+// first cut's measures of the steps, by other workgroups.
+template <typename R>
+__device__ __forceinline__ Prefix cut(Shared& sh, const R& row, const Plan& plan, List& list, float hi, const u64* given) {
+    const Prefix all = plan.all;
+    Prefix kept = all;
+    if (plan.by_count) {
+        const Search<R, Step> search = {sh, row, plan.weigh, plan.step, true, all};
+        auto want_of = [&](u64) { return (u64)plan.k; };
+        if (given || plan.k <= THREADS / 2) {
+            if (given) {
+                load(sh, given, NB);
+            } else {
+                // the threads' largest tokens alone bound the k-th of all: what lies in
+                // their k-th's step or above is few
+                clear(sh);
+                if (hi > all.x) atomicAdd(&sh.hist[plan.step(hi)], 1ull);
+            }
+            locate(sh, want_of);
+            const int bin = sh.bin;
+            if (bin < NB - 1) list.n = row.list(sh, [&](int i, float x) { return (plan.step(x) <= bin) & all.has(x, i); });
+        }
+        if (list.n > NB) {
+            kept = search(want_of, given);
+            list.n = row.list(sh, [&](int i, float x) { return kept.has(x, i); });
+            if (list.n <= NB) kept = all;
+        } else {
+            const Search<List, Step> among = {sh, list, plan.weigh, plan.step, true, all};
+            kept = among(want_of);
+        }
+    }
+    if (plan.by_mass) {
+        auto want_of = [&](u64 sum) { return share(plan.p, sum); };
+        if (list.n > NB) {
+            const Search<R, Step> search = {sh, row, plan.weigh, plan.step, false, kept};
+            const u64 want = search.divide(want_of, plan.by_count ? nullptr : given);
+            const int bin = sh.bin;
+            const u64 above = sh.above;
+            if (bin < NB - 1) {
+                list.n = row.list(sh, [&](int i, float x) { return (plan.step(x) <= bin) & kept.has(x, i); });
+                if (list.n <= NB) {
+                    const Search<List, Step> among = {sh, list, plan.weigh, plan.step, false, all};
+                    kept = among.within(bin, above, want);
+                } else {
+                    kept = search.within(bin, above, want);
+                }
+            }
+        } else {
+            const Search<List, Step> among = {sh, list, plan.weigh, plan.step, false, kept};
+            kept = among(want_of);
+        }
+    }
+    return kept;
 }
 
-template <bool F32, bool FEW>
-__global__ void __launch_bounds__(THREADS, 8) smg_sample_t(SampleArgs a) {
-    __shared__ Shared sh;
-    const int r = blockIdx.x, tid = threadIdx.x;
-    Row<F32, FEW> row;
-    row.init(a);
-
-    float lo = INFINITY, hi = -INFINITY;
+// (smallest above -inf, largest) of the tokens, over the workgroup; hi: this thread's
+template <typename R>
+__device__ __forceinline__ float2 ends_of(Shared& sh, const R& row, float& hi) {
+    float lo = INFINITY;
+    hi = -INFINITY;
     row.each([&](int, float x) {
         hi = fmaxf(hi, x);  // NaN is passed over
         lo = fminf(lo, x > -INFINITY ? x : lo);
     });
-    const float2 ends = block_range(sh, lo, hi);
-    const float t = a.temperature[r];
-    if (ends.y == -INFINITY) {
-        if (tid == 0) a.out[r] = -1;
+    return block_range(sh, lo, hi);
+}
+template <typename R>
+__device__ __forceinline__ int first_of(Shared& sh, const R& row, float largest) {
+    int first = 0x7fffffff;
+    if (threadIdx.x == 0) sh.index = 0x7fffffff;
+    row.each([&](int i, float x) { first = min(first, x == largest ? i : 0x7fffffff); });
+    __syncthreads();
+    if (first != 0x7fffffff) atomicMin(&sh.index, first);
+    __syncthreads();
+    return sh.index;
+}
+
+template <bool F32, bool FEW>
+__global__ void __launch_bounds__(THREADS) smg_sample_t(SampleArgs a) {
+    __shared__ Shared sh;
+    const int r = blockIdx.x;
+    Row<F32, FEW> row;
+    row.init(a, r);
+    float hi;
+    const float2 ends = ends_of(sh, row, hi);
+    Plan plan(a, r);
+    int found = -1;
+    if (ends.y > -INFINITY && !(plan.t > 0.f)) {
+        found = first_of(sh, row, ends.y);
+    } else if (ends.y > -INFINITY) {
+        plan.init(sh, a, r, ends);
+        List list = {&sh, NB + 1};
+        const Prefix kept = cut(sh, row, plan, list, hi, nullptr);
+        if (list.n <= NB)
+            found = sh.list_i[plan.draw<true>(sh, list, kept)];
+        else if (plan.by_count || plan.by_mass)
+            found = plan.draw<true>(sh, row, kept);
+        else
+            found = plan.draw<false>(sh, row, kept);
+    }
+    if (threadIdx.x == 0) a.out[r] = found;
+}
+
+// ---- few long rows: workgroups share a row, in five launches ---------------------
+// Each of the passes over a row that cost the most (the largest logit, the first cut's
+// measures, the last sums) has `parts` workgroups a row; the searches between them have
+// one.  Integer sums make the answer the same.
+__device__ __forceinline__ float2 ends_of(const Work& w, int parts) {
+    const int lane = threadIdx.x & 63;
+    const float lo = lane < parts ? w.lo[lane] : INFINITY, hi = lane < parts ? w.hi[lane] : -INFINITY;
+    return make_float2(-wave_max(-lo), wave_max(hi));
+}
+
+template <bool F32>
+__global__ void __launch_bounds__(THREADS) smg_sample_ends_t(SampleArgs a) {
+    __shared__ Shared sh;
+    const int part = blockIdx.x, r = blockIdx.y;
+    Work& w = ((Work*)a.work)[r];
+    Row<F32, false> row;
+    row.init(a, r, part, a.parts);
+    for (int i = part * THREADS + threadIdx.x; i < NB; i += a.parts * THREADS) w.hist[i] = 0;
+    float hi;
+    const float2 ends = ends_of(sh, row, hi);
+    const int first = a.temperature[r] > 0.f ? 0 : first_of(sh, row, ends.y);
+    if (threadIdx.x == 0) w.lo[part] = ends.x, w.hi[part] = ends.y, w.first[part] = first;
+}
+
+// the first cut's measures, or without a cut the last sums
+template <bool F32>
+__global__ void __launch_bounds__(THREADS) smg_sample_measure_t(SampleArgs a) {
+    __shared__ Shared sh;
+    const int part = blockIdx.x, r = blockIdx.y;
+    Work& w = ((Work*)a.work)[r];
+    const float2 ends = ends_of(w, a.parts);
+    Plan plan(a, r);
+    if (ends.y == -INFINITY || !(plan.t > 0.f)) return;
+    plan.init(sh, a, r, ends);
+    Row<F32, false> row;
+    row.init(a, r, part, a.parts);
+    if (!plan.by_count && !plan.by_mass) {
+        __syncthreads();
+        row.sums(w.blocks, [&](int i, float x) { return plan.template left<false>(plan.all, i, x); });
         return;
     }
-    if (!(t > 0.f)) {
-        int first = 0x7fffffff;
-        if (tid == 0) sh.index = 0x7fffffff;
-        row.each([&](int i, float x) { first = min(first, x == ends.y ? i : 0x7fffffff); });
-        __syncthreads();
-        if (first != 0x7fffffff) atomicMin(&sh.index, first);
-        __syncthreads();
-        if (tid == 0) a.out[r] = sh.index;
-        return;
-    }
-    Weigh weigh;
-    weigh.init(sh, ends.y, t, a.V);
+    const Search<Row<F32, false>, Step> search = {sh, row, plan.weigh, plan.step, plan.by_count, plan.all};
+    search.fill();
+    __syncthreads();
+    for (int i = threadIdx.x; i < NB; i += THREADS)
+        if (sh.hist[i]) atomicAdd(&w.hist[i], sh.hist[i]);
+}
 
-    // steps down from the largest: to the smallest, or to where weights are 0
-    // (below 2^-51), whose tokens the last step takes
-    const float cap = weigh.cap;
-    const float depth = fminf(cap - ends.x, 51.f * 0.69314718f * t);
-    const float per = depth > 1e-30f ? (NB - 2) / depth : 0.f;
-    auto step = [&](float x) { return (int)fminf((cap - fminf(x, cap)) * per, NB - 1.f); };
+template <bool F32>
+__global__ void __launch_bounds__(THREADS) smg_sample_cut_t(SampleArgs a) {
+    __shared__ Shared sh;
+    const int r = blockIdx.x;
+    Work& w = ((Work*)a.work)[r];
+    const float2 ends = ends_of(w, a.parts);
+    Plan plan(a, r);
+    Row<F32, false> row;
+    row.init(a, r);
+    int found = -1;
+    bool open = false;
+    if (ends.y > -INFINITY && !(plan.t > 0.f)) {
+        for (int part = a.parts - 1; part >= 0; --part)
+            if (w.hi[part] == ends.y) found = w.first[part];
+    } else if (ends.y > -INFINITY) {
+        plan.init(sh, a, r, ends);
+        if (!plan.by_count && !plan.by_mass) {
+            found = plan.draw<false>(sh, row, plan.all, w.blocks);
+        } else {
+            List list = {&sh, NB + 1};
+            const Prefix kept = cut(sh, row, plan, list, 0.f, w.hist);
+            open = list.n > NB;
+            if (open)
+                w.x = kept.x, w.i = kept.i;
+            else
+                found = sh.list_i[plan.draw<true>(sh, list, kept)];
+        }
+    }
+    if (threadIdx.x == 0) {
+        w.open = open;
+        a.out[r] = found;
+    }
+}
 
-    // everything above -inf, or the +inf
-    const Prefix all = {ends.y == INFINITY ? cap : -INFINITY, -1};
-    Prefix kept = all;
-    const int k = a.top_k ? a.top_k[r] : 0;
-    const float p = a.top_p ? a.top_p[r] : 1.f;
-    const float mp = a.min_p ? a.min_p[r] : 0.f;
-    const float u = a.u[r];
-    const bool by_count = k > 0 && k < a.V, by_mass = p < 1.f;
-    List list = {&sh, NB + 1};
-    if (by_count) {
-        Search<Row<F32, FEW>, decltype(step)> search = {sh, row, weigh, step, true, all};
-        if (k <= THREADS / 2) {
-            // the threads' largest tokens alone bound the k-th of all: what lies in
-            // their k-th's step or above is few
-            clear(sh);
-            if (hi > all.x) atomicAdd(&sh.hist[step(hi)], 1ull);
-            locate(sh, [&](u64) { return (u64)k; });
-            const int bin = sh.bin;
-            if (bin < NB - 1) list.n = row.list(sh, [&](int i, float x) { return (step(x) <= bin) & all.has(x, i); });
-        }
-        if (list.n > NB) {
-            kept = search([&](u64) { return (u64)k; });
-            list.n = row.list(sh, [&](int i, float x) { return kept.has(x, i); });
-            if (list.n <= NB) kept = all;
-        } else {
-            Search<List, decltype(step)> among = {sh, list, weigh, step, true, all};
-            kept = among([&](u64) { return (u64)k; });
-        }
-    }
-    if (by_mass) {
-        auto want_of = [&](u64 sum) { return share(p, sum); };
-        if (list.n > NB) {
-            Search<Row<F32, FEW>, decltype(step)> search = {sh, row, weigh, step, false, kept};
-            const u64 want = search.divide(want_of);
-            const int bin = sh.bin;
-            const u64 above = sh.above;
-            if (bin < NB - 1) {
-                list.n = row.list(sh, [&](int i, float x) { return (step(x) <= bin) & kept.has(x, i); });
-                if (list.n <= NB) {
-                    Search<List, decltype(step)> among = {sh, list, weigh, step, false, all};
-                    kept = among.within(bin, above, want);
-                } else {
-                    kept = search.within(bin, above, want);
-                    list.n = NB + 1;
-                }
-            }
-        } else {
-            Search<List, decltype(step)> among = {sh, list, weigh, step, false, kept};
-            kept = among(want_of);
-        }
-    }
-    int found;
-    if (list.n <= NB) {
-        found = sh.list_i[draw<true>(sh, list, weigh, kept, u, mp)];
-    } else if (by_count || by_mass) {
-        found = draw<true>(sh, row, weigh, kept, u, mp);
-    } else {
-        found = draw<false>(sh, row, weigh, kept, u, mp);
-    }
-    if (tid == 0) a.out[r] = found;
+// the last sums of the rows that are still open
+template <bool F32>
+__global__ void __launch_bounds__(THREADS) smg_sample_sums_t(SampleArgs a) {
+    __shared__ Shared sh;
+    const int part = blockIdx.x, r = blockIdx.y;
+    Work& w = ((Work*)a.work)[r];
+    if (!w.open) return;
+    Plan plan(a, r);
+    plan.init(sh, a, r, ends_of(w, a.parts));
+    __syncthreads();
+    Row<F32, false> row;
+    row.init(a, r, part, a.parts);
+    const Prefix kept = {w.x, w.i};
+    row.sums(w.blocks, [&](int i, float x) { return plan.template left<true>(kept, i, x); });
+}
+
+template <bool F32>
+__global__ void __launch_bounds__(THREADS) smg_sample_pick_t(SampleArgs a) {
+    __shared__ Shared sh;
+    const int r = blockIdx.x;
+    Work& w = ((Work*)a.work)[r];
+    if (!w.open) return;
+    Plan plan(a, r);
+    plan.init(sh, a, r, ends_of(w, a.parts));
+    Row<F32, false> row;
+    row.init(a, r);
+    const int found = plan.draw<true>(sh, row, {w.x, w.i}, w.blocks);
+    if (threadIdx.x == 0) a.out[r] = found;
 }
 
 template <bool F32>
 void launch(const SampleArgs& a, hipStream_t s) {
-    if (a.V < 8)
+    if (a.V < 8) {
         hipLaunchKernelGGL((smg_sample_t<F32, true>), dim3(a.R), dim3(THREADS), 0, s, a);
-    else
+    } else if (a.parts == 1) {
         hipLaunchKernelGGL((smg_sample_t<F32, false>), dim3(a.R), dim3(THREADS), 0, s, a);
+    } else {
+        const dim3 all(a.parts, a.R);
+        hipLaunchKernelGGL(smg_sample_ends_t<F32>, all, dim3(THREADS), 0, s, a);
+        hipLaunchKernelGGL(smg_sample_measure_t<F32>, all, dim3(THREADS), 0, s, a);
+        hipLaunchKernelGGL(smg_sample_cut_t<F32>, dim3(a.R), dim3(THREADS), 0, s, a);
+        if (a.top_k || a.top_p) {
+            hipLaunchKernelGGL(smg_sample_sums_t<F32>, all, dim3(THREADS), 0, s, a);
+            hipLaunchKernelGGL(smg_sample_pick_t<F32>, dim3(a.R), dim3(THREADS), 0, s, a);
+        }
+    }
 }
 
 }  // namespace
 
+// bytes of workspace that a row takes where workgroups share it
+extern "C" long long smg_sample_work_bytes() { return (long long)sizeof(Work); }
+
 extern "C" int smg_sample_launch(const void* logits, const void* u, const void* temperature,
                                  const void* top_k, const void* top_p, const void* min_p, void* out,
-                                 long long stride, int R, int V, int f32, void* stream) {
-    if (V < 1 || V > MAX_V) return -1;
+                                 void* work, long long stride, int R, int V, int parts, int f32, void* stream) {
+    if (V < 1 || V > MAX_V || parts < 1 || parts > MAX_PARTS || (parts > 1 && (!work || R > 65535))) return -1;
     if (R < 1) return 0;
     SampleArgs a = {logits, stride, (const float*)u, (const float*)temperature, (const int*)top_k,
-                    (const float*)top_p, (const float*)min_p, (long long*)out, R, V};
+                    (const float*)top_p, (const float*)min_p, (long long*)out, R, V, (u64*)work, parts};
     if (f32)
         launch<true>(a, (hipStream_t)stream);
     else

@@ -501,10 +501,13 @@ class TestSample:
         x = randn(g, len(US), V, dtype=torch.float32 if f32 else BF16, scale=2.0)
         check_sample(x, US, [1.0, 0.6, 1.4, 0.0, 1.0, 0.8, 2.0, 0.3, 1.0], k, p, m)
 
-    def test_mixed_rows(self):
+    @pytest.mark.parametrize("R,V", [(300, 5000), (60, 70001), (128, 65536), (129, 65536)])
+    def test_mixed_rows(self, R, V):
         g = gen(1)
-        R = 300
-        x = randn(g, R, 5000, scale=3.0)
+        x = randn(g, R, V, scale=3.0)
+        x[R // 2] = -math.inf
+        x[R // 3, V // 2:] = -math.inf
+        x[R // 4, 3] = x[R // 4, V - 1] = math.inf
         pick = lambda *v: [v[i] for i in torch.randint(0, len(v), (R,), generator=g, device=DEV).tolist()]  # noqa: E731
         check_sample(x, torch.rand(R, generator=g, device=DEV).tolist(), pick(0.0, 0.5, 1.0, 1.5), pick(0, 1, 7, 300, 9000),
                      pick(0.0, 0.1, 0.9, 0.99, 1.0), pick(0.0, 0.001, 0.1, 1.0))
