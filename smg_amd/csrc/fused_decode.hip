@@ -121,6 +121,8 @@ extern "C" __global__ void __launch_bounds__(256) smg_silu_mul(
 // layout sdpa wants (so the flash prefill consumes them with zero transpose
 // copies).  Replaces the per-layer torch chain: 2x rope complex-mul chains,
 // 2x advanced-index KV scatter, and the implicit transpose-contiguous copies.
+// Without a cache (null k_cache) it only rotates: drafted tokens' K/V stay out
+// of the cache until they are accepted.
 template <bool KV8>
 __global__ void __launch_bounds__(WAVE) smg_rope_prefill_t(
     const __hip_bfloat16* __restrict__ qkv,   // [B, L, D + 2*KD]
@@ -182,6 +184,7 @@ __global__ void __launch_bounds__(WAVE) smg_rope_prefill_t(
         const __hip_bfloat16 v1 = vrow[e + 1];
         vo[e] = v0;
         vo[e + 1] = v1;
+        if (!k_cache) continue;
         if constexpr (KV8) {
             store_pair_fp8(kc8 + e, krf0, krf1);
             store_pair_fp8(vc8 + e, __bfloat162float(v0), __bfloat162float(v1));

@@ -24,6 +24,8 @@ import numpy as np
 import torch
 import torch.nn.functional as F
 
+from . import ops
+
 
 @dataclass
 class TorchEngineConfig:
@@ -56,6 +58,10 @@ class TorchEngineConfig:
     # Requires the gfx950 fused kernels.  Default OFF — the bench headline
     # is measured with the bf16 cache.
     kv_fp8: bool = False
+    # opt-in packed prefill: prompts and chunks of different lengths and
+    # histories share one forward (ops.attn_prefill) instead of waiting for
+    # others of their length.  Requires the gfx950 kernels.
+    packed_prefill: bool = False
 
     @classmethod
     def tiny(cls) -> "TorchEngineConfig":
@@ -136,11 +142,35 @@ def _rms(x, weight):
     return F.rms_norm(x, (x.shape[-1],), weight=weight, eps=1e-5)
 
 
+GREEDY = (0.0, 0, 1.0, 0.0)  # (temperature, top_k, top_p, min_p)
+
+
+def _sampling_of(temperature, top_k, top_p, min_p) -> tuple:
+    """A request's sampling settings, checked; GREEDY for temperature 0."""
+    s = (float(temperature), max(0, int(top_k)), float(top_p), float(min_p))
+    if not (0 <= s[0] < math.inf and 0 < s[2] <= 1 and 0 <= s[3] <= 1 and s[1] < 2 ** 31):
+        raise ValueError(f"sampling needs a temperature >= 0, an int32 top_k, 0 < top_p <= 1 and 0 <= min_p <= 1, got {s}")
+    return s if s[0] > 0 else GREEDY
+
+
+def _sample_cpu(logits, u, temperature, top_k, top_p, min_p):
+    """ops.sample for the CPU logic tests, in plain torch."""
+    x, t = logits.double(), temperature.double()[:, None]
+    w, order = ((x - x.amax(-1, keepdim=True)) / torch.where(t > 0, t, 1.0)).exp().sort(dim=-1, descending=True, stable=True)
+    place = torch.arange(x.shape[1])
+    w = torch.where((place < top_k[:, None]) | (top_k[:, None] <= 0), w, 0.0)
+    before = w.cumsum(-1) - w
+    w = torch.where((before < top_p[:, None] * w.sum(-1, keepdim=True)) | (place == 0) | (top_p[:, None] >= 1), w, 0.0)
+    w = torch.where((w >= min_p[:, None]) | (place == 0), w, 0.0)
+    w = torch.zeros_like(w).scatter_(1, order, w).cumsum(-1)
+    return torch.where(t[:, 0] > 0, (w <= u[:, None] * w[:, -1:]).sum(-1), order[:, 0])
+
+
 class _Request:
     __slots__ = ("rid", "tokens", "max_new", "slot", "prefilled", "generated", "done",
-                 "prefill_only", "pc_keys", "mm_embed", "await_embed")
+                 "prefill_only", "pc_keys", "mm_embed", "await_embed", "sampling")
 
-    def __init__(self, rid, tokens, max_new, prefill_only=False):
+    def __init__(self, rid, tokens, max_new, prefill_only=False, sampling=GREEDY):
         self.rid = rid
         self.tokens = tokens
         self.max_new = max_new
@@ -152,6 +182,7 @@ class _Request:
         self.pc_keys = None  # prefix-cache chain keys, precomputed at submit
         self.mm_embed = None  # [E, d_model] EPD vision embeddings (seq prefix)
         self.await_embed = False  # EPD: hold prefill until accept_embed pairs
+        self.sampling = sampling  # (temperature, top_k, top_p, min_p)
 
 
 class TorchEngine:
@@ -193,6 +224,12 @@ class TorchEngine:
         self._gen_cnt = np.zeros(c.max_slots, dtype=np.int64)  # len(generated) per slot
         self._maxnew_arr = np.zeros(c.max_slots, dtype=np.int64)
         self._last_tok = torch.zeros(c.max_slots, dtype=torch.long, device=self.device)
+        # sampling settings of the slots' requests (GREEDY where they have none)
+        self._sampling_host: List[tuple] = [GREEDY] * c.max_slots
+        self._sampling = tuple(torch.full((c.max_slots,), v, dtype=d, device=self.device)
+                               for v, d in zip(GREEDY, (torch.float32, torch.int32, torch.float32, torch.float32)))
+        self._sampling_used = False  # by any request so far
+        self._sampling_gen = torch.Generator(device=self.device).manual_seed(c.seed + 1)
         self._arange_slots = torch.arange(c.max_slots, device=self.device)
         self._free_slots = list(range(c.max_slots - 1, -1, -1))
         self.waiting: List[_Request] = []
@@ -346,9 +383,21 @@ class TorchEngine:
                 " rope_kv_store/rope_prefill/attn_decode) on a CUDA/HIP device"
             )
 
+        if c.packed_prefill and not self._has_ops():
+            raise RuntimeError(
+                "packed_prefill=True requires the gfx950 kernels (smg_amd._core) on a CUDA/HIP"
+                f" device, bfloat16 and a head dim of {ops.HEAD_DIMS}"
+            )
+
+    def _has_ops(self) -> bool:
+        """Whether attention over the cache runs on the kernels of ops.py."""
+        return (self._hip_fused is not None and getattr(self, "_hip_rope_prefill", None) is not None
+                and self.cfg.head_dim in ops.HEAD_DIMS)
+
     # ---- API -------------------------------------------------------------
     def submit(self, tokens: List[int], max_new_tokens: int, rid: Optional[str] = None,
-               prefill_only: bool = False, mm_embed=None, await_embed: bool = False) -> str:
+               prefill_only: bool = False, mm_embed=None, await_embed: bool = False,
+               temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0) -> str:
         """`prefill_only` is the PD prefill leg: the request prefills, samples
         its first token (emitted with the PREFILLED flag, value 4) and PARKS —
         the slot stays allocated until export_kv() hands its KV off to the
@@ -360,7 +409,12 @@ class TorchEngine:
         vision-tower embeddings that occupy sequence positions 0..E-1 in
         front of the prompt tokens (the reference ships these engine-side
         via Mooncake after the encode fleet runs; here they arrive over the
-        xGMI plane — comm/plane.py EMB transfer directions)."""
+        xGMI plane — comm/plane.py EMB transfer directions).
+
+        `temperature` above 0 samples the request's tokens (ops.sample) with
+        `top_k` (0: all), `top_p` (1: all) and `min_p` (0: none) from the
+        engine's own generator; 0 takes the likeliest token."""
+        sampling = _sampling_of(temperature, top_k, top_p, min_p)
         if rid is None:
             self._rid_counter += 1
             rid = f"req-{self._rid_counter}"
@@ -380,7 +434,9 @@ class TorchEngine:
             keep = max(1, c.max_seq - 2 - n_emb)
             toks = toks[-keep:]  # keep the prompt tail
         max_new_tokens = max(1, min(max_new_tokens, c.max_seq - 1 - len(toks) - n_emb))
-        req = _Request(rid, toks, max_new_tokens, prefill_only=prefill_only)
+        self._sampling_used |= sampling[0] > 0
+        req = _Request(rid, toks, max_new_tokens, prefill_only=prefill_only,
+                       sampling=sampling)
         if mm_embed is None:
             # EPD decode leg: embeddings that arrived over the plane
             # (accept_embed) pair with the request by rid
@@ -422,18 +478,23 @@ class TorchEngine:
         self._requests.pop(rid, None)
         return t, plen, first_tok
 
-    def import_kv(self, rid, kv_tensor, plen: int, first_tok: int, max_new: int) -> bool:
+    def import_kv(self, rid, kv_tensor, plen: int, first_tok: int, max_new: int,
+                  temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0) -> bool:
         """Decode-leg intake: place the transferred KV into a free slot and
-        continue decoding from the prefill-sampled first token."""
+        continue decoding from the prefill-sampled first token, with the
+        sampling settings of submit()."""
+        sampling = _sampling_of(temperature, top_k, top_p, min_p)
         if not self._free_slots:
             return False
         c = self.cfg
         slot = self._free_slots.pop()
         self.kv[:, :, slot, :, :plen] = kv_tensor.to(self.kv.dtype)
+        self._sampling_used |= sampling[0] > 0
+        self._set_sampling(slot, sampling)
         self._seq_len_host[slot] = plen
         self.seq_len[slot] = plen
         self._last_tok[slot] = int(first_tok)
-        req = _Request(rid, [0] * plen, max_new)  # token VALUES unused post-prefill
+        req = _Request(rid, [0] * plen, max_new, sampling=sampling)  # token VALUES unused post-prefill
         req.prefilled = plen
         req.slot = slot
         req.generated = [int(first_tok)]
@@ -494,7 +555,7 @@ class TorchEngine:
         """Launch one engine iteration WITHOUT reading results back.
 
         All admission/completion control flow here is host-deterministic —
-        "done" is a token-COUNT condition and sampling is argmax payload — so
+        "done" is a token-COUNT condition and the chosen token is payload — so
         the sampled token VALUES are only event payload.  They are copied
         device→pinned-slab asynchronously and read in step_finish().  The
         pipelined TickGateway resolves tick N-1's handle while tick N's
@@ -513,6 +574,7 @@ class TorchEngine:
             self._seq_len_host[req.slot] = 0
             self._gen_cnt[req.slot] = len(req.generated)
             self._maxnew_arr[req.slot] = req.max_new
+            self._set_sampling(req.slot, req.sampling)
 
         h = _StepHandle()
         samples: List[tuple] = []  # (device tensor, slab base offset)
@@ -579,24 +641,38 @@ class TorchEngine:
                    and not r.await_embed]
         if pending:
             pending.sort(key=lambda sr: len(sr[1].tokens) - sr[1].prefilled)
+        if pending and c.packed_prefill:
+            # the shortest first, each as far as the tokens of a forward go
+            group, lens, room = [], [], int(c.prefill_budget_mult * c.prefill_chunk)
+            for slot, req in pending[: c.prefill_group]:
+                n = min(len(req.tokens) - req.prefilled, c.prefill_chunk, room)
+                if n <= 0:
+                    break
+                group.append((slot, req))
+                lens.append(n)
+                room -= n
+        elif pending:
             min_rem = len(pending[0][1].tokens) - pending[0][1].prefilled
             L = min(min_rem, c.prefill_chunk)
             group = [sr for sr in pending if len(sr[1].tokens) - sr[1].prefilled >= L][: c.prefill_group]
             # keep the total under the budget multiple
             while len(group) > 1 and len(group) * L > c.prefill_budget_mult * c.prefill_chunk:
                 group.pop()
+            lens = [L] * len(group)
+        if pending:
             items = []
-            for slot, req in group:
-                items.append((slot, req.prefilled, req.tokens[req.prefilled: req.prefilled + L]))
+            for (slot, req), n in zip(group, lens):
+                items.append((slot, req.prefilled, req.tokens[req.prefilled: req.prefilled + n]))
             t2 = _t()
-            nxt_pf = self._prefill_batch(items)  # device [len(group)]
+            # device [len(group)]
+            nxt_pf = self._prefill_packed(items) if c.packed_prefill else self._prefill_batch(items)
             lt["pf"] += _t() - t2
             pf_off = off
             samples.append((nxt_pf, pf_off))
             off += len(items)
             finished_pf = []
             for i, (slot, req) in enumerate(group):
-                req.prefilled += L
+                req.prefilled += lens[i]
                 if req.prefilled >= len(req.tokens):
                     self._prefix_store(slot, req.tokens)
                     if req.prefill_only:
@@ -746,6 +822,31 @@ class TorchEngine:
                             pin_memory=self.device.type == "cuda")
             self._slabs[self._slab_i] = s
         return s
+
+    # ---- sampling ----------------------------------------------------------
+    def _set_sampling(self, slot: int, sampling: tuple) -> None:
+        if self._sampling_host[slot] != sampling:
+            self._sampling_host[slot] = sampling
+            for t, v in zip(self._sampling, sampling):
+                t[slot] = v
+
+    def _samples(self) -> bool:
+        """Whether a running request samples: all greedy, the forwards end in an argmax."""
+        return self._sampling_used and any(r.sampling[0] > 0 for r in self.running.values())
+
+    def _choose(self, logits: torch.Tensor, slots: Optional[torch.Tensor] = None, each: int = 1) -> torch.Tensor:
+        """The next token of each row of logits, for all slots or `each` rows a slot of
+        `slots` in turn, by the settings of the slots' requests."""
+        if not self._samples():
+            return logits.argmax(-1)
+        u = torch.rand(logits.shape[0], generator=self._sampling_gen, device=self.device)
+        given = self._sampling if slots is None else tuple(t[slots].repeat_interleave(each) for t in self._sampling)
+        if self.device.type != "cuda":
+            return _sample_cpu(logits, u, *given)
+        if logits.dtype not in (torch.bfloat16, torch.float32):
+            logits = logits.float()
+        temperature, top_k, top_p, min_p = given
+        return ops.sample(logits, u, temperature, top_k=top_k, top_p=top_p, min_p=min_p)
 
     # ---- forwards ----------------------------------------------------------
     def _kv_hist(self, li: int, which: int, slots):
@@ -1004,6 +1105,8 @@ class TorchEngine:
             return False
         if B < 4:  # singles/tiny groups: capture overhead isn't worth it
             return False
+        if self._samples():  # the captured forwards end in an argmax
+            return False
         # graphable paths: cold flash-causal, or uniform-start suffix merge
         if fresh:
             return True
@@ -1197,10 +1300,152 @@ class TorchEngine:
         # For requests whose prefill completes with this chunk this IS the
         # first generated token; for the rest _last_tok is overwritten by
         # their final chunk before decode ever reads it.
-        nxt = (_rms(h[:, -1], self.ln_f) @ self.embed.t()).argmax(-1)  # [B]
+        nxt = self._choose(_rms(h[:, -1], self.ln_f) @ self.embed.t(), slots)  # [B]
         self._last_tok[slots] = nxt
         self.seq_len[slots] = starts + L
         return nxt  # device tensor: the caller defers (or performs) the D2H read
+
+    def _rope_rows(self, qkv, slots, pos, k_out, v_out, cache=None) -> torch.Tensor:
+        """Rotary embedding of rows of a fused projection [N, D + 2 KD], each at a
+        slot and position of its own (int32 [N]): q [N, heads, head_dim] comes back,
+        k and v go to k_out, v_out [N, kv heads, head_dim] and, where one layer's
+        `cache` (K, V) is given, to the rows' places in it."""
+        c = self.cfg
+        q = torch.empty(qkv.shape[0], c.n_heads, c.head_dim, device=self.device, dtype=self.dtype)
+        k_cache, v_cache = (t.data_ptr() for t in cache) if cache else (0, 0)
+        self._hip_rope_prefill(
+            qkv.data_ptr(), self.freqs_cis.data_ptr(), slots.data_ptr(), pos.data_ptr(),
+            k_cache, v_cache, q.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
+            qkv.shape[0], 1, c.n_heads, c.max_seq, c.head_dim, torch.cuda.current_stream().cuda_stream,
+            1 if self.kv.dtype == torch.float8_e4m3fn else 0, c.kv_heads,
+        )
+        return q
+
+    @torch.no_grad()
+    def _prefill_packed(self, items: List[tuple]) -> torch.Tensor:
+        """Prefill of `items` = [(slot, start, tokens)] of any lengths and histories in
+        one forward over their packed tokens; returns the sampled tokens ([len(items)],
+        device)."""
+        c = self.cfg
+        lens = np.asarray([len(toks) for _, _, toks in items], dtype=np.int64)
+        slots_np = np.asarray([s for s, _, _ in items], dtype=np.int64)
+        starts_np = np.asarray([st for _, st, _ in items], dtype=np.int64)
+        ends = np.cumsum(lens)
+        N, B = int(ends[-1]), len(items)
+        cu_np = np.concatenate([[0], ends])
+        pos_np = np.arange(N) - np.repeat(cu_np[:-1] - starts_np, lens)
+        # one transfer: tokens | slot and position of each | slots, starts, offsets, last rows
+        meta = self._h2d_i64(np.concatenate([
+            np.concatenate([toks for _, _, toks in items]), np.repeat(slots_np, lens), pos_np,
+            slots_np, starts_np, cu_np, ends - 1])).clone()
+        t, row_slots, row_pos, slots, starts, cu, last = meta.split([N, N, N, B, B, B + 1, B])
+        small = meta[N:].to(torch.int32)
+        row_slots32, row_pos32, slots32, starts32, cu32, _ = small.split([N, N, B, B, B + 1, B])
+        h = self.embed[t]  # [N, D]
+        kb = torch.empty(N, c.kv_heads, c.head_dim, device=self.device, dtype=self.dtype)
+        vb = torch.empty_like(kb)
+        max_ctx = int((starts_np + lens).max())
+        for li, layer in enumerate(self.layers):
+            k, v = self.kv[li, 0], self.kv[li, 1]
+            q = self._rope_rows(_rms(h, layer.ln1) @ layer.wqkv, row_slots32, row_pos32, kb, vb, (k, v))
+            attn = ops.attn_prefill(q, k, v, slots32, starts32, cu32, max_ctx=max_ctx)
+            h = torch.addmm(h, attn.view(N, c.d_model), layer.wo)
+            h = self._mlp(h, layer)
+        nxt = self._choose(_rms(h[last], self.ln_f) @ self.embed.t(), slots)
+        self._last_tok[slots] = nxt
+        self.seq_len[slots] = starts + (cu[1:] - cu[:-1])
+        for (slot, start, toks) in items:
+            self._seq_len_host[slot] = int(start) + len(toks)
+        return nxt
+
+    @torch.no_grad()
+    def step_drafts(self, drafts: Dict[str, tuple]) -> Dict[str, List[int]]:
+        """Verifies drafted continuations of running requests in one forward.
+
+        `drafts` maps a request to (tokens, parents): drafted tokens and, for each, the
+        index of the drafted token that it follows, which comes before it, or -1 where
+        it follows the request's last token; at most ops.MAX_NODES - 1 of them.  The
+        model's token after every node is chosen as the request's settings have it; a
+        draft is accepted where it is that token.  Every request gains the accepted
+        tokens and one more, which come back by request (and as events); requests
+        that are not running with their prompt prefilled are refused, and so is a step
+        launched and not yet finished.
+
+        The drafts' K/V stay out of the cache until they are accepted (ops.attn_tree,
+        ops.tree_commit).  Synchronous: the accepted counts decide what is done."""
+        c = self.cfg
+        if not self._has_ops():
+            raise RuntimeError("step_drafts requires the gfx950 kernels (smg_amd._core) on a CUDA/HIP device,"
+                               f" bfloat16 and a head dim of {ops.HEAD_DIMS}")
+        by_rid = {r.rid: (s, r) for s, r in self.running.items() if r.prefilled >= len(r.tokens)}
+        rows = []
+        for rid, (tokens, parents) in drafts.items():
+            if rid not in by_rid:
+                raise KeyError(f"{rid} is not running with its prompt prefilled")
+            if len(tokens) != len(parents) or len(tokens) >= ops.MAX_NODES:
+                raise ValueError(f"{rid}: {len(tokens)} drafts and {len(parents)} parents, at most {ops.MAX_NODES - 1} of each")
+            if any(not -1 <= p < i for i, p in enumerate(parents)):
+                raise ValueError(f"{rid}: a parent comes before its child, or is -1")
+            slot, req = by_rid[rid]
+            if len(req.generated) != self._gen_cnt[slot] or (req.generated and req.generated[-1] < 0):
+                raise RuntimeError(f"{rid}: a launched step has to be finished first")
+            # node 0 is the request's last token; drafts beyond the cache are left out
+            depth = [0]
+            for p in parents:
+                depth.append(depth[p + 1] + 1)
+            room = c.max_seq - 1 - int(self._seq_len_host[slot])
+            up = [-1] + [p + 1 if d <= room else -2 for p, d in zip(parents, depth[1:])]
+            rows.append((slot, req, [0] + [int(t) % c.vocab_size for t in tokens], up, depth))
+        if not rows:
+            return {}
+        B, N = len(rows), max(len(r[2]) for r in rows)
+        pad = lambda v, x: v + [x] * (N - len(v))  # noqa: E731
+        tree = np.asarray([[pad(t, 0), pad(up, -2), pad([d if u >= -1 else 0 for d, u in zip(depth, up)], 0)]
+                           for _, _, t, up, depth in rows], dtype=np.int64)
+        slots_np = np.asarray([r[0] for r in rows], dtype=np.int64)
+        meta = self._h2d_i64(np.concatenate([tree.ravel(), slots_np])).clone()
+        tree_t, slots = meta[:-B].view(B, 3, N), meta[-B:]
+        tokens = tree_t[:, 0].contiguous()
+        tokens[:, 0] = self._last_tok[slots]
+        parents = tree_t[:, 1].to(torch.int32).contiguous()
+        ctx = self.seq_len[slots]
+        pos = (ctx[:, None] + tree_t[:, 2]).to(torch.int32).view(-1)
+        row_slots = slots.to(torch.int32).repeat_interleave(N)
+        slots32, ctx32 = slots.to(torch.int32), ctx.to(torch.int32)
+        max_ctx = int(self._seq_len_host[slots_np].max())
+        kv_new = torch.empty(c.n_layers, 2, B, N, c.kv_heads, c.head_dim, device=self.device, dtype=self.dtype)
+        h = self.embed[tokens.view(-1)]
+        for li, layer in enumerate(self.layers):
+            q = self._rope_rows(_rms(h, layer.ln1) @ layer.wqkv, row_slots, pos, kv_new[li, 0], kv_new[li, 1])
+            attn = ops.attn_tree(q.view(B, N, c.n_heads, c.head_dim), kv_new[li, 0], kv_new[li, 1],
+                                 self.kv[li, 0], self.kv[li, 1], slots32, ctx32, parents, max_ctx=max_ctx)
+            h = torch.addmm(h, attn.view(B * N, c.d_model), layer.wo)
+            h = self._mlp(h, layer)
+        targets = self._choose(_rms(h, self.ln_f) @ self.embed.t(), slots, each=N).view(B, N)
+        count, path, nxt = ops.tree_commit(kv_new, self.kv, slots32, ctx32, parents, tokens, targets)
+        self._last_tok[slots] = nxt
+        self.seq_len[slots] += count
+        out, freed = {}, []
+        taken = targets.gather(1, path.clamp_min(0).long()).tolist()
+        for (slot, req, *_), n, toks in zip(rows, count.tolist(), taken):
+            got = toks[: min(n, req.max_new - len(req.generated))]
+            req.generated.extend(got)
+            self._gen_cnt[slot] = len(req.generated)
+            self._seq_len_host[slot] += n
+            self.total_generated += len(got)
+            req.done = len(req.generated) >= req.max_new or self._seq_len_host[slot] >= c.max_seq - 2
+            for i, t in enumerate(got):
+                self._step_events.append((req.rid, t, 1 if req.done and i == len(got) - 1 else 0))
+            out[req.rid] = got
+            if req.done:
+                freed.append(slot)
+        for s in freed:
+            del self.running[s]
+            self._free_slots.append(s)
+            self._seq_len_host[s] = 0
+        if freed:
+            self.seq_len[self._h2d_i64(np.asarray(freed, dtype=np.int64))] = 0
+        return out
 
     def _decode_core(self, maxlen: int) -> torch.Tensor:
         """Full-arena decode forward: every slot participates with a static
@@ -1245,8 +1490,7 @@ class TorchEngine:
             h = h + attn_flat @ layer.wo
             h = self._mlp(h, layer)
         h = _rms(h, self.ln_f)
-        logits = h[:, 0] @ self.embed.t()
-        return logits.argmax(-1)  # [S]
+        return self._choose(h[:, 0] @ self.embed.t())  # [S]
 
     @torch.no_grad()
     def _decode_core_fused(self) -> torch.Tensor:
@@ -1307,7 +1551,7 @@ class TorchEngine:
             self._hip_silu_mul(gu.data_ptr(), self._smul_buf.data_ptr(), S, c.d_ffn, stream)
             h = torch.addmm(h, self._smul_buf, layer.w2)
         h = _rms(h, self.ln_f)
-        return (h @ self.embed.t()).argmax(-1)  # [S]
+        return self._choose(h @ self.embed.t())  # [S]
 
     GRAPH_BUCKET = 256
 
@@ -1353,7 +1597,7 @@ class TorchEngine:
 
         maxlen = int(self._seq_len_host.max()) + 1
         if (self.graphs and self.device.type == "cuda"
-                and not _os.environ.get("SMG_NO_DECODE_GRAPH")):
+                and not _os.environ.get("SMG_NO_DECODE_GRAPH") and not self._samples()):
             nxt = self._decode_graphed(maxlen)
         else:
             nxt = self._decode_core(maxlen)

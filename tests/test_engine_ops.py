@@ -750,3 +750,205 @@ class TestTogether:
             again = ops.attn_prefill(q[b, taken].contiguous(), kv[0, 0], kv[0, 1], slots[b:b + 1], ctx[b:b + 1], i32([0, len(taken)]))
             # both within the two roundings of the 64-bit value
             assert (again.float() - out[b, taken].float()).abs().max() <= 4 * HALF * out.abs().max().float()
+
+
+def engine(device=DEV, **kw):
+    from smg_amd.engine.torch_engine import TorchEngine, TorchEngineConfig
+
+    cfg = TorchEngineConfig.tiny()
+    for k, v in kw.items():
+        setattr(cfg, k, v)
+    return TorchEngine(cfg, device=device)
+
+
+def run(eng, *rids):
+    for _ in range(300):
+        if all(eng.finished(r) for r in rids):
+            break
+        eng.step()
+    return [eng.collect(r) for r in rids]
+
+
+class TestEngineSampling:
+    @pytest.mark.parametrize("device", ["cpu", pytest.param(DEV, marks=pytest.mark.gpu)])
+    def test_requests_have_their_own_settings(self, device):
+        eng, ref = engine(device), engine(device)
+        prompts = [[i * 7 + j for j in range(12)] for i in range(3)]
+        want = run(ref, *[ref.submit(p, 6) for p in prompts])
+        # a sampled request beside greedy ones; top_k 1 and a tiny top_p leave the likeliest
+        a = eng.submit(prompts[0], 6)
+        b = eng.submit(prompts[1], 6, temperature=1.5, top_k=1)
+        c = eng.submit(prompts[2], 6, temperature=0.7, top_p=1e-6)
+        assert run(eng, a, b, c) == want
+        # its slot is greedy again afterwards
+        assert run(eng, *[eng.submit(p, 6) for p in prompts]) == want
+
+    @pytest.mark.parametrize("device", ["cpu", pytest.param(DEV, marks=pytest.mark.gpu)])
+    def test_draws_differ_and_repeat(self, device):
+        outs = []
+        for _ in range(2):
+            eng = engine(device)
+            outs.append(run(eng, *[eng.submit(list(range(9)), 8, temperature=2.0) for _ in range(4)]))
+        assert outs[0] == outs[1]  # the engine's generator starts from its seed
+        assert len({tuple(o) for o in outs[0]}) > 1
+        assert all(0 <= t < 2048 for o in outs[0] for t in o)
+
+    def test_refusals(self):
+        eng = engine("cpu")
+        for kw in (dict(temperature=-1.0), dict(temperature=math.inf), dict(top_p=0.0), dict(top_p=1.5), dict(min_p=-0.1), dict(min_p=2.0), dict(top_k=1 << 31)):
+            with pytest.raises(ValueError):
+                eng.submit([1, 2], 2, **kw)
+
+    def test_settings_follow_the_kv(self):
+        a, b = engine("cpu"), engine("cpu")
+        rid = a.submit(list(range(30)), 8, prefill_only=True, temperature=2.0)
+        a.step()
+        kv, plen, first = a.export_kv(rid)
+        with pytest.raises(ValueError):
+            b.import_kv(rid, kv, plen, first, 8, temperature=-1.0)
+        assert b.import_kv(rid, kv, plen, first, 8, temperature=1.5, top_k=1)
+        c = engine("cpu")
+        assert c.import_kv(rid, kv, plen, first, 8)
+        assert run(b, rid) == run(c, rid)
+
+    def test_kernels_are_asked_for_on_cpu(self):
+        with pytest.raises(RuntimeError, match="packed_prefill"):
+            engine("cpu", packed_prefill=True)
+        eng = engine("cpu")
+        with pytest.raises(RuntimeError, match="step_drafts"):
+            eng.step_drafts({})
+
+
+def kv_rows(eng, slot, n):
+    return eng.kv[:, :, slot, :, :n].float()
+
+
+@pytest.mark.gpu
+class TestEnginePaths:
+    @pytest.mark.parametrize("kw", [{}, dict(n_kv_heads=2), dict(n_kv_heads=2, kv_fp8=True), dict(prefill_chunk=24, prefill_budget_mult=1.0)])
+    def test_packed_prefill_fills_the_cache_as_the_batched_one(self, kw):
+        base = dict(kw)
+        base.pop("prefill_chunk", None), base.pop("prefill_budget_mult", None)
+        g = torch.Generator().manual_seed(0)
+        prompts = [torch.randint(0, 2048, (n,), generator=g).tolist() for n in (5, 130, 1, 64, 97)]
+        prompts.append(prompts[1][:64] + [7, 8, 9])  # a prefix-cache hit once prompt 1 is stored
+        packed, plain = engine(packed_prefill=True, **kw), engine(**base)
+        for eng in (packed, plain):
+            for p in prompts[:5]:
+                eng.submit(p, 90, rid=str(len(p)))
+            for _ in range(30):
+                eng.step()
+            eng.submit(prompts[5], 90, rid="hit")
+            for _ in range(20):
+                eng.step()
+            assert eng.prefix_cache_hits >= 1
+        slots = [{r.rid: s for s, r in eng.running.items()} for eng in (packed, plain)]
+        for p in prompts:
+            rid = "hit" if p is prompts[5] else str(len(p))
+            a, b = (kv_rows(eng, sl[rid], len(p)) for eng, sl in zip((packed, plain), slots))
+            # the layers' inputs differ by roundings of the layer before: bf16 steps (8-bit
+            # ones of the cached K/V) of values up to a few units
+            assert (a - b).abs().max() <= (0.3 if kw.get("kv_fp8") else 0.06) * max(1.0, b.abs().max().item())
+            first = [eng._requests[rid].generated[0] for eng in (packed, plain)]
+            assert all(0 <= t < 2048 for t in first)
+
+    @pytest.mark.parametrize("kw", [{}, dict(n_kv_heads=1), dict(n_kv_heads=2, kv_fp8=True)])
+    def test_drafts_are_verified_and_committed(self, kw):
+        eng = engine(**kw)
+        prompts = [list(range(3, 40)), list(range(100, 105))]
+        rids = [eng.submit(p, 40) for p in prompts]
+        while any(r.prefilled < len(r.tokens) for r in eng.waiting + list(eng.running.values())):
+            eng.step()
+        before = {r: list(eng._requests[r].generated) for r in rids}
+        # what the model chooses after each node comes back; drafted again, it is accepted
+        got = eng.step_drafts({r: ([], []) for r in rids})
+        assert all(len(v) == 1 for v in got.values())
+        for _ in range(4):
+            probe = {}
+            for r in rids:
+                # wrong guesses beside each other, and a chain below one of them
+                probe[r] = ([1, 2, 3, 4], [-1, -1, 1, 2])
+            more = eng.step_drafts(probe)
+            for r in rids:
+                got[r] += more[r]
+        events = {}
+        for r, t, _ in eng.drain_events():
+            events.setdefault(r, []).append(t)
+        for r in rids:
+            req = eng._requests[r]
+            assert req.generated == before[r] + got[r] and events[r][-len(got[r]):] == got[r]
+            # the cache holds the tokens but the last, as a prefill of them does
+            tokens = prompts[rids.index(r)] + req.generated[:-1]
+            slot = req.slot
+            assert eng._seq_len_host[slot] == len(tokens) == eng.seq_len[slot].item()
+            ref = engine(**kw)
+            rr = ref.submit(tokens, 2)
+            ref.step()
+            a, b = kv_rows(eng, slot, len(tokens)), kv_rows(ref, ref._requests[rr].slot, len(tokens))
+            assert (a - b).abs().max() <= (0.3 if kw.get("kv_fp8") else 0.06) * max(1.0, b.abs().max().item())
+
+    def test_right_drafts_are_accepted(self):
+        engs = [engine(), engine()]
+        rids = [e.submit(list(range(50)), 30) for e in engs]
+        for e, rid in zip(engs, rids):
+            while not e._requests[rid].generated:
+                e.step()
+        # the first engine's choice is drafted, twice, in the second one
+        nxt = engs[0].step_drafts({rids[0]: ([], [])})[rids[0]][0]
+        eng, rid = engs[1], rids[1]
+        slot = eng._requests[rid].slot
+        n = int(eng._seq_len_host[slot])
+        got = eng.step_drafts({rid: ([(nxt + 1) % 2048, nxt, nxt, 5], [-1, -1, -1, 1])})[rid]
+        assert got[0] == nxt and len(got) >= 2
+        assert eng.seq_len[slot].item() == n + len(got) == eng._seq_len_host[slot]
+        assert eng._last_tok[slot].item() == got[-1]
+
+    def test_drafts_end_with_the_request(self):
+        eng = engine()
+        rid = eng.submit(list(range(20)), 3)
+        while not eng._requests[rid].generated:
+            eng.step()
+        for _ in range(3):
+            if eng.finished(rid):
+                break
+            eng.step_drafts({rid: ([1, 2], [-1, 0])})
+        assert eng.finished(rid) and len(eng.collect(rid)) == 3
+        assert len(eng._free_slots) == eng.cfg.max_slots
+        flags = [d for r, _, d in eng.drain_events() if r == rid]
+        assert flags[-1] == 1 and not any(flags[:-1])
+
+    def test_drafts_at_the_end_of_the_cache(self):
+        eng = engine(max_seq=64)
+        rid = eng.submit(list(range(55)), 100)
+        while not eng._requests[rid].generated:
+            eng.step()
+        while not eng.finished(rid):
+            eng.step_drafts({rid: (list(range(20)), [i - 1 for i in range(20)])})
+        assert len(eng._free_slots) == eng.cfg.max_slots
+
+    def test_draft_refusals(self):
+        eng = engine()
+        rid = eng.submit(list(range(20)), 9)
+        with pytest.raises(KeyError):
+            eng.step_drafts({rid: ([], [])})  # not prefilled yet
+        while not eng._requests[rid].generated:
+            eng.step()
+        for tokens, parents in (([1], []), ([1], [0]), ([1, 2], [-1, 1]), ([1], [-2]), ([1] * 64, [-1] * 64)):
+            with pytest.raises(ValueError):
+                eng.step_drafts({rid: (tokens, parents)})
+        assert eng.step_drafts({}) == {}
+        handle = eng.step_launch()
+        with pytest.raises(RuntimeError, match="finished"):
+            eng.step_drafts({rid: ([], [])})
+        eng.step_finish(handle)
+        assert eng.step_drafts({rid: ([], [])})[rid]
+
+    def test_sampled_drafts(self):
+        eng = engine(n_kv_heads=2)
+        rids = [eng.submit(list(range(9 * i, 9 * i + 9)), 20, temperature=t, top_p=0.9) for i, t in enumerate((0.0, 1.0, 0.5))]
+        while any(not eng._requests[r].generated for r in rids):
+            eng.step()
+        for _ in range(5):
+            got = eng.step_drafts({r: ([3, 4], [-1, -1]) for r in rids})
+            eng.step()  # and decoding goes on in between
+            assert all(got.values())
