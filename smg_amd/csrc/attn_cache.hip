@@ -23,7 +23,7 @@
 // (ds_read_b64_tr_b16 gives a lane 4 consecutive key rows of one column).  P
 // never leaves the registers, and m, l and the rescaling are per lane.  P is
 // rounded to bf16 because the matrix cores take no wider second operand at
-// this rate: at most 2^-9 relative a weight, while l sums the f32 values.
+// this rate: at most 2^-8 relative a weight, while l sums the f32 values.
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>
 
@@ -770,8 +770,9 @@ int launch(const AttnArgs& a, int D, int wr, hipStream_t s) {
     return D == 128 ? launch_d<TREE, KV8, 128>(a, wr, s) : D == 64 ? launch_d<TREE, KV8, 64>(a, wr, s) : -1;
 }
 
-int bad_shape(int H, int KVH, int S, int T, int n_split) {
+int bad_shape(long long rows, int H, int KVH, int S, int T, int n_split) {
     if (KVH <= 0 || H <= 0 || H % KVH) return -4;
+    if (rows * H > 1 << 30 || T > 1 << 30) return -5;  // row and key numbers are 32 bits
     if (S <= 0 || T <= 0 || n_split < 1) return -3;
     return 0;
 }
@@ -783,7 +784,7 @@ extern "C" int smg_attn_prefill_launch(
     const void* q, const void* k, const void* v, const void* slots, const void* ctx, const void* cu,
     void* out, void* part_o, void* part_ml, const long long* strides, int B, int N, int H, int KVH,
     int S, int T, int D, int n_split, int wr, float scale, int kv_fp8, void* stream) {
-    if (int rc = bad_shape(H, KVH, S, T, n_split)) return rc;
+    if (int rc = bad_shape(N, H, KVH, S, T, n_split)) return rc;
     if (B < 1 || N < 1) return 0;
     AttnArgs a = {};
     a.q = (const __hip_bfloat16*)q;
@@ -810,7 +811,7 @@ extern "C" int smg_attn_tree_launch(
     const void* slots, const void* ctx, const void* parents, void* out, void* part_o, void* part_ml,
     const long long* strides, int B, int N, int H, int KVH, int S, int T, int D, int n_split, int wr,
     float scale, int kv_fp8, void* stream) {
-    if (int rc = bad_shape(H, KVH, S, T, n_split)) return rc;
+    if (int rc = bad_shape((long long)B * N, H, KVH, S, T, n_split)) return rc;
     if (N > 64) return -3;
     if (B < 1 || N < 1) return 0;
     AttnArgs a = {};

@@ -546,8 +546,8 @@ __device__ __forceinline__ u64 share(float p, u64 all) {  // the measure that to
 }
 
 struct Step {
-    float cap, per;
-    __device__ __forceinline__ int operator()(float x) const { return (int)fminf((cap - fminf(x, cap)) * per, NB - 1.f); }
+    float cap, half, per;  // halves, whose differences stay in range
+    __device__ __forceinline__ int operator()(float x) const { return (int)fminf(fmaf(fminf(x, cap), -.5f, half) * per, NB - 1.f); }
 };
 
 // A row's settings, and what follows from its largest and smallest logit.
@@ -572,8 +572,8 @@ struct Plan {
         weigh.init(sh, ends.y, t, a.V);
         // steps down from the largest: to the smallest, or to where weights are 0
         // (below 2^-51), whose tokens the last step takes
-        const float depth = fminf(weigh.cap - ends.x, 51.f * 0.69314718f * t);
-        step = {weigh.cap, depth > 1e-30f ? (NB - 2) / depth : 0.f};
+        const float half = .5f * weigh.cap, depth = fminf(fmaf(ends.x, -.5f, half), .5f * 51.f * 0.69314718f * t);
+        step = {weigh.cap, half, depth > 1e-30f ? (NB - 2) / depth : 0.f};
         all = {ends.y == INFINITY ? weigh.cap : -INFINITY, -1};
         const float mp = a.min_p ? a.min_p[r] : 0.f;
         least = mp > 0.f ? fmin((double)mp, 1.) * weigh.units : 0.;

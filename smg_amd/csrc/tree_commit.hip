@@ -72,9 +72,10 @@ __global__ void __launch_bounds__(256) smg_tree_commit_t(CommitArgs a) {
         if (lane == cur) a.next[b] = len ? target : -1;
     }
     if (!len) return;
-    // of entries that name one slot the last writes it
+    // of entries that name one slot the last that is no padding writes it
     bool later = false;
-    for (int i = b + 1 + lane; i < a.B; i += WAVE) later |= a.slots[i] == slot;
+    for (int i = b + 1 + lane; i < a.B; i += WAVE)
+        if (a.slots[i] == slot) later |= a.ctx[i] >= 0 && a.ctx[i] < a.T && a.parents[(size_t)i * a.N] == -1;
     if (__any(later)) return;
 
     const int chunks = a.D / 8;

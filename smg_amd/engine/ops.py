@@ -9,6 +9,9 @@ bfloat16 or float8_e4m3fn; its dimensions may have any strides but the last,
 which is dense.  Rows of tensors that kernels read 16 bytes at a time start at
 multiples of 16 bytes (8 where tree_commit writes an 8-bit cache).
 
+They are forwards without a gradient, for a worker that answers: a first argument
+that asks for one is refused where gradients are recorded.
+
 What the host cannot see is bounded on the device: a sequence whose slot lies
 outside the cache is a padding entry, lengths and offsets are cut to the tensors.
 """
@@ -77,7 +80,7 @@ def _cache(k: torch.Tensor, v: torch.Tensor, dev: int, H: int, D: int) -> tuple:
         raise ValueError(f"k_cache {tuple(shape)} {k.dtype} and v_cache {tuple(v.shape)} {v.dtype} differ")
     if d != D or D not in HEAD_DIMS:
         raise ValueError(f"head dim must be one of {HEAD_DIMS} and equal, got {D} over a cache of {d}")
-    if S < 1 or KVH < 1 or T < 1 or H < 1 or H % KVH:
+    if S < 1 or KVH < 1 or not 1 <= T <= 1 << 30 or H < 1 or H % KVH:
         raise ValueError(f"{H} heads over a cache of {tuple(shape)}")
     return S, KVH, T, _rows("k_cache", k) + _rows("v_cache", v)
 
@@ -95,12 +98,14 @@ def _out(out: Optional[torch.Tensor], q: torch.Tensor, dev: int) -> torch.Tensor
     if out is None:
         return torch.empty_like(q, memory_format=torch.contiguous_format)
     _check("out", out, (_BF16,), q.dim(), dev)
-    if out.shape != q.shape:
-        raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
+    if out.shape != q.shape or 0 in out.stride():
+        raise ValueError(f"out must be {tuple(q.shape)} with a place for every element, got {tuple(out.shape)} with strides {out.stride()}")
     return out
 
 
 def _on_gpu(name: str, t: torch.Tensor, dev: int) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name} asks for a gradient, and the operators have none: detach it or use torch.no_grad()")
     if dev < 0:
         raise RuntimeError(f"{name} is on {t.device}: the operators run on a CUDA/HIP device")
     if _core is None:
@@ -156,7 +161,7 @@ def attn_prefill(
 
     max_ctx, a bound on starts[b] plus the new tokens, only sizes the split of
     long caches over the card (default: the cache's length).  Returns out
-    [N, H, D]; rows that no sequence covers are not written.  A sequence whose slot
+    [N, H, D], which may be q itself; rows that no sequence covers are not written.  A sequence whose slot
     lies outside the cache gets zeros."""
     _check("q", q, (_BF16,), 3, None)
     dev = q.get_device()
@@ -172,6 +177,8 @@ def attn_prefill(
     _on_gpu("q", q, dev)
     if N == 0 or B == 0:
         return out
+    if N * H > 1 << 30:
+        raise ValueError(f"at most {1 << 30} rows of a head, got {N} x {H}")
     total = N * (H // KVH)
     fp8 = k_cache.dtype is _FP8
     wr = _waves(total // B, D, fp8)
@@ -199,7 +206,7 @@ def attn_tree(
     sequence whose slot lies outside the cache.
 
     max_ctx, a bound on ctx_lens, only sizes the split of long caches over the
-    card (default: the cache's length)."""
+    card (default: the cache's length).  Returns out [B, N, H, D], which may be q."""
     _check("q", q, (_BF16,), 4, None)
     dev = q.get_device()
     B, N, H, D = q.shape
@@ -219,6 +226,8 @@ def attn_tree(
     _on_gpu("q", q, dev)
     if B == 0 or N == 0:
         return out
+    if B * N * H > 1 << 30:
+        raise ValueError(f"at most {1 << 30} rows of a head, got {B} x {N} x {H}")
     rows = N * (H // KVH)
     fp8 = k_cache.dtype is _FP8
     wr = _waves(rows, D, fp8)
@@ -248,8 +257,8 @@ def tree_commit(
     Returns (count int32 [B], path int32 [B, N], next int64 [B]): how many nodes
     were taken, which (-1 after the last), and the last one's target, the
     sequence's next token.  A sequence whose slot lies outside the cache, that has
-    no room or whose node 0 has a parent is padding: 0, -1, -1.  Of sequences that
-    name the same slot the last one's rows are written."""
+    no room or whose node 0 has a parent is padding: 0, -1, -1.  Of other sequences
+    that name the same slot the last one's rows are written."""
     _check("kv_new", kv_new, (_BF16,), 6, None)
     dev = kv_new.get_device()
     L, two, B, N, KVH, D = kv_new.shape
@@ -259,6 +268,8 @@ def tree_commit(
         raise ValueError(f"kv_new {tuple(kv_new.shape)} does not fit kv_cache {tuple(kv_cache.shape)}")
     if D % 8:
         raise ValueError(f"head dim must be a multiple of 8, got {D}")
+    if 0 in kv_cache.stride():
+        raise ValueError(f"kv_cache must have a place for every element, strides {kv_cache.stride()}")
     if N > MAX_NODES or (N < 1 and B > 0):
         raise ValueError(f"1 to {MAX_NODES} drafted nodes, got {N}")
     strides = _rows("kv_new", kv_new) + _rows("kv_cache", kv_cache, 16 if kv_cache.dtype is _BF16 else 8)

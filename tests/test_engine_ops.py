@@ -123,6 +123,13 @@ class TestAttnPrefill:
         check_prefill(out, qs, kt, layers[1, 1], slots, st, cu, scale=0.03)
         assert (wide[:, 1::2] == 7).all()
 
+    @pytest.mark.parametrize("lens,starts", [([70, 1, 9], [0, 30, 500]), ([3], [6000])])
+    @pytest.mark.parametrize("fp8", [False, True])
+    def test_out_may_be_q(self, lens, starts, fp8):
+        q, *rest = prefill_case(lens, starts, 8, 2, 128, fp8, seed=9)
+        want = ops.attn_prefill(q, *rest)
+        assert ops.attn_prefill(q, *rest, out=q) is q and torch.equal(q, want)
+
     def test_rows_behind_the_last_sequence_stay(self):
         for starts in ([3, 5], [3, 4000]):  # without and with a split
             q, k, v, slots, st, cu = prefill_case([30, 10], starts, 4, 2, 128, seed=5)
@@ -348,19 +355,20 @@ def commit_plain(kv_new, kv, slots, ctx, parents, tokens, targets):
     kv = kv.clone()
     S, T = kv.shape[2], kv.shape[4]
     B, N = parents.shape
+    real = [0 <= c < T and up == -1 for c, up in zip(ctx.tolist(), parents[:, 0].tolist())]
     count, path, nxt = [], [], []
     for b in range(B):
         p, tk, tg = parents[b].tolist(), tokens[b].tolist(), targets[b].tolist()
         slot, at = slots[b].item(), ctx[b].item()
         taken = []
-        if 0 <= slot < S and 0 <= at < T and p[0] == -1:
+        if 0 <= slot < S and real[b]:
             taken = [0]
             while len(taken) < T - at:
                 below = [c for c in range(taken[-1] + 1, N) if p[c] == taken[-1] and tk[c] == tg[taken[-1]]]
                 if not below:
                     break
                 taken.append(below[0])
-            if taken and slot not in slots[b + 1:].tolist():
+            if not any(r and s == slot for r, s in zip(real[b + 1:], slots[b + 1:].tolist())):
                 kv[:, :, slot, :, at:at + len(taken)] = kv_new[:, :, b, taken].transpose(2, 3).to(kv.dtype)
         count.append(len(taken))
         path.append(taken + [-1] * (N - len(taken)))
@@ -410,6 +418,13 @@ class TestTreeCommit:
         args = commit_case(2, 4, 1, 64, seed=4)
         args[4][0, 0] = -2
         assert check_commit(args)[0] == 0
+
+    def test_padding_may_name_a_used_slot(self):
+        args = commit_case(5, 6, 2, 64, T=40, seed=9)
+        args[2] = i32([3, 3, 3, 3, 3])  # one real entry, and three kinds of padding behind it
+        args[3] = i32([2, 7, 40, -1, 9])
+        args[4][4, 0] = -2
+        assert check_commit(args)[2:] == [0, 0, 0]
 
     def test_same_slot_twice(self):
         args = commit_case(70, 6, 2, 64, seed=5)
@@ -572,6 +587,12 @@ class TestSample:
             x[:, 11] = 3.4e38
             check_sample(x, US, math.inf, k=9, p=0.7)
             check_sample(x, US, 1.0, k=9, p=0.7)
+        # from one end of the type to the other, at temperatures that leave all a weight
+        x = (torch.rand(len(US), 5000, generator=gen(9), device=DEV) - 0.5) * 6.8e38
+        assert (x.amax(1) - x.amin(1)).isinf().all()
+        for t in (3e38, math.inf):
+            check_sample(x, US, t, k=4000, p=0.7)
+            check_sample(x, US, t, p=0.999)
         x = randn(gen(8), len(US), 5000, dtype=torch.float32, scale=1e-42)  # denormals
         check_sample(x, US, 1.0, k=100, p=0.5)
 
@@ -681,6 +702,12 @@ class TestRefusals:
         ("commit", dict(kn=torch.zeros(1, 2, 2, 3, 2, 12, dtype=BF16), kv=torch.zeros(1, 2, 4, 2, 16, 12, dtype=BF16)), ValueError),
         ("commit", dict(tokens=torch.zeros(2, 3, dtype=torch.int32)), TypeError),
         ("commit", dict(targets=torch.zeros(3, 2, dtype=torch.int64)), ValueError),
+        ("prefill", dict(out=torch.zeros(1, 4, 64, dtype=BF16).expand(6, 4, 64)), ValueError),
+        ("commit", dict(kv=torch.zeros(1, 2, 1, 2, 16, 64, dtype=BF16).expand(1, 2, 4, 2, 16, 64)), ValueError),
+        ("prefill", dict(q=torch.zeros(6, 4, 64, dtype=BF16, requires_grad=True)), RuntimeError),
+        ("tree", dict(q=torch.zeros(2, 3, 4, 64, dtype=BF16, requires_grad=True)), RuntimeError),
+        ("commit", dict(kn=torch.zeros(1, 2, 2, 3, 2, 64, dtype=BF16, requires_grad=True)), RuntimeError),
+        ("sample", dict(logits=torch.zeros(2, 9, requires_grad=True)), RuntimeError),
         ("sample", dict(logits=torch.zeros(2, 9, dtype=torch.float16)), TypeError),
         ("sample", dict(logits=torch.zeros(9)), ValueError),
         ("sample", dict(logits=torch.zeros(2, 0)), ValueError),
