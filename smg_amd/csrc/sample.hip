@@ -34,11 +34,13 @@
 #define WAVE 64
 #define THREADS 1024
 #define WAVES (THREADS / WAVE)
-#define NB 2048             // steps of a histogram; also the most blocks and listed tokens
+#define NB 2048             // steps of a histogram; also the most blocks
+#define LIST 8192           // most listed tokens
 #define BLOCK 512           // tokens of a wave's iteration
 #define CAND 128            // tokens that are compared with each other
 #define MAX_V (NB * BLOCK)
-#define DEEP 2              // loads of a wave on their way
+#define DEEP 2              // loads of a wave on their way in a pass that computes
+#define LIGHT 4             // and in one that only compares
 #define MAX_PARTS 16        // workgroups of a row
 
 namespace {
@@ -74,8 +76,8 @@ struct Work {
 
 struct Shared {
     u64 hist[NB];
-    float list_x[NB];
-    int list_i[NB];
+    float list_x[LIST];
+    int list_i[LIST];
     double pow2[64];  // 2^(i/64 + S)
     u64 part[WAVES];
     float lo[WAVES], hi[WAVES];
@@ -160,20 +162,17 @@ __device__ __forceinline__ void load(Shared& sh, const u64* from, int n) {
     for (int i = threadIdx.x; i < NB; i += THREADS) sh.hist[i] = i < n ? from[i] : 0;
 }
 
-// Adds the NB counters of sh.hist up: sh.bin and sh.above get the first at which
-// the sum reaches want(sum of all) and the sum before it (bin NB if it never
-// does).  Returns that want.
-template <typename W>
-__device__ __forceinline__ u64 locate(Shared& sh, W&& want_of) {
-    constexpr int OWN = NB / THREADS;  // counters of a thread
+// Adds numbers up, of which thread t has the sums sum[] of the first 1, 2, .. of its own,
+// number `own` * t and so on: sh.bin and sh.above get the first number at which the sum
+// reaches want(sum of all) and the sum before it (bin NONE if it never does).  Returns
+// that want.
+#define NONE 0x7fffffff
+template <int OWN, typename W>
+__device__ __forceinline__ u64 locate(Shared& sh, const u64 (&sum)[OWN], int own, W&& want_of) {
     const int t = threadIdx.x;
-    __syncthreads();
-    u64 sum[OWN];
-#pragma unroll
-    for (int i = 0; i < OWN; ++i) sum[i] = sh.hist[OWN * t + i] + (i ? sum[i - 1] : 0);
     const u64 run = wave_scan(sum[OWN - 1]);
     if ((t & 63) == 63) sh.part[t / WAVE] = run;
-    if (t == 0) sh.bin = NB;
+    if (t == 0) sh.bin = NONE;
     __syncthreads();
     u64 all;
     const u64 before = before_wave(sh.part, &all) + run - sum[OWN - 1];
@@ -184,11 +183,21 @@ __device__ __forceinline__ u64 locate(Shared& sh, W&& want_of) {
 #pragma unroll
         for (int i = 0; i < OWN - 1; ++i)
             if (before + sum[i] < want) n = i + 1, above = before + sum[i];
-        sh.bin = OWN * t + n;
+        sh.bin = own * t + n;
         sh.above = above;
     }
     __syncthreads();
     return want;
+}
+// the same of the NB counters of sh.hist
+template <typename W>
+__device__ __forceinline__ u64 locate(Shared& sh, W&& want_of) {
+    constexpr int OWN = NB / THREADS;
+    __syncthreads();
+    u64 sum[OWN];
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) sum[i] = sh.hist[OWN * threadIdx.x + i] + (i ? sum[i - 1] : 0);
+    return locate(sh, sum, OWN, want_of);
 }
 
 // the order's tokens up to the value x, of those equal to x up to index i
@@ -286,6 +295,9 @@ struct Row {
         }
         return r;
     }
+    __device__ __forceinline__ float value(int i) const {
+        return __uint_as_float(F32 ? ((const unsigned*)at)[i] : (unsigned)((const unsigned short*)at)[i] << 16);
+    }
     // row r, or part `part` of `parts` of it
     __device__ __forceinline__ void init(const SampleArgs& a, int r, int part = 0, int parts = 1) {
         lane = threadIdx.x & 63;
@@ -302,23 +314,23 @@ struct Row {
 #pragma unroll
         for (int e = 0; e < 8; ++e) f(b + e, r[e]);
     }
-    // g(it, raw) for each iteration that has tokens: DEEP loads at once
-    template <typename G>
+    // g(it, raw) for each iteration that has tokens: ON_WAY loads at once
+    template <int ON_WAY = DEEP, typename G>
     __device__ __forceinline__ void blocks(G&& g) const {
         const int n = min(its, (end - start + BLOCK - 1) / BLOCK);
-        for (int i0 = 0; i0 < n; i0 += DEEP) {
-            Raw r[DEEP];
+        for (int i0 = 0; i0 < n; i0 += ON_WAY) {
+            Raw r[ON_WAY];
 #pragma unroll
-            for (int i = 0; i < DEEP; ++i)
+            for (int i = 0; i < ON_WAY; ++i)
                 if (i0 + i < n) r[i] = load8(i0 + i);
 #pragma unroll
-            for (int i = 0; i < DEEP; ++i)
+            for (int i = 0; i < ON_WAY; ++i)
                 if (i0 + i < n) g(i0 + i, r[i]);
         }
     }
-    template <typename F>
+    template <int ON_WAY = DEEP, typename F>
     __device__ __forceinline__ void each(F&& f) const {
-        blocks([&](int it, const Raw& r) { each8(it, r, f); });
+        blocks<ON_WAY>([&](int it, const Raw& r) { each8(it, r, f); });
     }
     // f(x, measure(i, x)) where that is not 0; the measures of 8 tokens side by side
     template <typename M, typename F>
@@ -371,30 +383,48 @@ struct Row {
         __syncthreads();
         return sh.index;
     }
+    // f(i, x) for the tokens that `rare`, a comparison that few pass
+    template <typename P, typename F>
+    __device__ __forceinline__ void some(P&& rare, F&& f) const {
+        blocks<LIGHT>([&](int it, const Raw& r) {
+            for (unsigned hits = these(it, r, [&](int, float x) { return rare(x); }); hits; hits &= hits - 1) {
+                const int i = base(it) + __ffs(hits) - 1;
+                f(i, value(i));
+            }
+        });
+    }
+    // a bit for each of an iteration's 8 tokens that `has`
+    template <typename H>
+    __device__ __forceinline__ unsigned these(int it, const Raw& r, H&& has) const {
+        unsigned hits = 0;
+        const int b = base(it);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) hits |= has(b + e, r[e]) ? 1u << e : 0u;
+        return hits;
+    }
     // Lists the tokens that `has` in index order, if they fit; their number.
     template <typename H>
     __device__ __forceinline__ int list(Shared& sh, H&& has) const {
         int c = 0;
-        each([&](int i, float x) { c += has(i, x); });
+        each<LIGHT>([&](int i, float x) { c += has(i, x); });
         c = __builtin_amdgcn_readlane(wave_scan(c), 63);
         __syncthreads();
         if (lane == 0) sh.ints[threadIdx.x / WAVE] = c;
         __syncthreads();
         int all, at = before_wave(sh.ints, &all);
-        if (all > NB || !c) {
+        if (all > LIST) {
             __syncthreads();
             return all;
         }
-        blocks([&](int it, const Raw& r) {
-            int n = 0;
-            each8(it, r, [&](int i, float x) { n += has(i, x); });
-            const int run = wave_scan(n);
+        if (c) blocks<LIGHT>([&](int it, const Raw& r) {
+            unsigned hits = these(it, r, has);
+            const int n = __popc(hits), run = wave_scan(n);
             int to = at + run - n;
             at += __builtin_amdgcn_readlane(run, 63);
-            if (n) each8(it, r, [&](int i, float x) {
-                if (has(i, x)) sh.list_x[to] = x, sh.list_i[to] = i, ++to;
-            });
+            for (; hits; hits &= hits - 1) sh.list_i[to++] = base(it) + __ffs(hits) - 1;
         });
+        __syncthreads();
+        for (int i = threadIdx.x; i < all; i += THREADS) sh.list_x[i] = value(sh.list_i[i]);
         __syncthreads();
         return all;
     }
@@ -403,16 +433,20 @@ struct Row {
 // The tokens that a cut left: i is their place in the list.
 struct List {
     static constexpr bool LISTED = true;
-    static constexpr int OWN = NB / THREADS;  // tokens of a thread
+    static constexpr int MOST = LIST / THREADS;  // tokens of a thread
     Shared* sh;
-    int n;
+    int n, own;
+    __device__ __forceinline__ void set(int tokens) { n = tokens, own = (n + THREADS - 1) / THREADS; }
+    __device__ __forceinline__ bool fits() const { return n <= LIST; }
     template <typename F>
     __device__ __forceinline__ void each(F&& f) const {
-#pragma unroll
-        for (int e = 0; e < OWN; ++e) {
-            const int i = OWN * threadIdx.x + e;
-            if (i < n) f(i, sh->list_x[i]);
-        }
+        for (int i = own * threadIdx.x, end = min(n, i + own); i < end; ++i) f(i, sh->list_x[i]);
+    }
+    template <typename P, typename F>
+    __device__ __forceinline__ void some(P&& rare, F&& f) const {
+        each([&](int i, float x) {
+            if (rare(x)) f(i, x);
+        });
     }
     template <typename M, typename F>
     __device__ __forceinline__ void weighed(M&& measure, F&& f) const {
@@ -423,13 +457,15 @@ struct List {
     }
     template <typename W, typename M>
     __device__ __forceinline__ int find(Shared& s, W&& want_of, M&& measure) const {
-        __syncthreads();
+        u64 sum[MOST];
 #pragma unroll
-        for (int e = 0; e < OWN; ++e) {
-            const int i = OWN * threadIdx.x + e;
-            s.hist[i] = i < n ? measure(i, s.list_x[i]) : 0;
+        for (int e = 0; e < MOST; ++e) {
+            const int i = own * threadIdx.x + e;
+            sum[e] = e ? sum[e - 1] : 0;
+            if (e < own && i < n) sum[e] += measure(i, s.list_x[i]);
         }
-        locate(s, want_of);
+        __syncthreads();
+        locate(s, sum, own, want_of);
         return s.bin;
     }
 };
@@ -460,7 +496,7 @@ struct Search {
             tokens.weighed([&](int i, float x) { return weigh.fixed(x, from.has(x, i)); },
                            [&](float x, u64 w) { atomicAdd(&sh.hist[step(x)], w); });
     }
-    // The step in which want(sum of all) is reached, NB - 1 or NB if it never is.
+    // The step in which want(sum of all) is reached, NB - 1 or more if it never is.
     template <typename W>
     __device__ __forceinline__ u64 divide(W&& want_of, const u64* given = nullptr) const {
         if (given)
@@ -472,7 +508,7 @@ struct Search {
     // The prefix, from the step `bin` in which `want` is reached and the measure
     // `above` it.
     __device__ __forceinline__ Prefix within(int bin, u64 above, u64 want) const {
-        float top = 0.f, bottom = 0.f;  // of the last division, if `again`
+        float top = step.highest(bin), bottom = step.lowest(bin);  // `again`: of the last division
         double c = 0.;
         bool again = false;
         for (;;) {
@@ -481,9 +517,8 @@ struct Search {
             if (threadIdx.x < CAND) sh.cand_before[threadIdx.x] = 0;
             __syncthreads();
             float lo = INFINITY, hi = -INFINITY;
-            tokens.each([&](int i, float x) {
-                const bool inside = again ? x >= bottom && x <= top && min(NB - 1, (int)(((double)top - (double)x) * c)) == bin : step(x) == bin;
-                if (!inside) return;
+            tokens.some([&](float x) { return (x >= bottom) & (x <= top); }, [&](int i, float x) {
+                if ((again ? min(NB - 1, (int)(((double)top - (double)x) * c)) : step(x)) != bin) return;
                 const u64 w = measure(i, x);
                 if (!w) return;
                 lo = fminf(lo, x), hi = fmaxf(hi, x);
@@ -548,6 +583,17 @@ __device__ __forceinline__ u64 share(float p, u64 all) {  // the measure that to
 struct Step {
     float cap, half, per;  // halves, whose differences stay in range
     __device__ __forceinline__ int operator()(float x) const { return (int)fminf(fmaf(fminf(x, cap), -.5f, half) * per, NB - 1.f); }
+    // values above -inf between which the tokens of the steps up to `bin`, or from it on,
+    // lie, and few others
+    __device__ __forceinline__ float lowest(int bin) const {
+        const double x = (double)cap - 2. * (bin + 1) / (double)per * (1. + 1e-6);
+        return fmaxf((float)(x - fabs(x) * 1e-6), -3.40282347e38f);
+    }
+    __device__ __forceinline__ float highest(int bin) const {
+        if (bin == 0) return INFINITY;
+        const double x = (double)cap - 2. * bin / (double)per * (1. - 1e-6);
+        return fmaxf((float)(x + fabs(x) * 1e-6), -3.40282347e38f);
+    }
 };
 
 // A row's settings, and what follows from its largest and smallest logit.
@@ -578,6 +624,8 @@ struct Plan {
         const float mp = a.min_p ? a.min_p[r] : 0.f;
         least = mp > 0.f ? fmin((double)mp, 1.) * weigh.units : 0.;
     }
+    // what the tokens of the steps up to `bin` reach
+    __device__ __forceinline__ float lowest(int bin) const { return all.x >= weigh.cap ? INFINITY : step.lowest(bin); }
     // the weights that `kept` and min-p leave
     template <bool CUT>
     __device__ __forceinline__ u64 left(Prefix kept, int i, float x) const {
@@ -601,7 +649,7 @@ struct Plan {
 };
 
 // Top-k, then top-p: what they keep, as a prefix of the list if that holds it
-// (list.n <= NB), else of the row.  hi: the largest of this thread's tokens; given: the
+// (list.fits()), else of the row.  hi: the largest of this thread's tokens; given: the
 // first cut's measures of the steps, by other workgroups.
 template <typename R>
 __device__ __forceinline__ Prefix cut(Shared& sh, const R& row, const Plan& plan, List& list, float hi, const u64* given) {
@@ -610,38 +658,43 @@ __device__ __forceinline__ Prefix cut(Shared& sh, const R& row, const Plan& plan
     if (plan.by_count) {
         const Search<R, Step> search = {sh, row, plan.weigh, plan.step, true, all};
         auto want_of = [&](u64) { return (u64)plan.k; };
-        if (given || plan.k <= THREADS / 2) {
-            if (given) {
-                load(sh, given, NB);
-            } else {
-                // the threads' largest tokens alone bound the k-th of all: what lies in
-                // their k-th's step or above is few
-                clear(sh);
-                if (hi > all.x) atomicAdd(&sh.hist[plan.step(hi)], 1ull);
-            }
+        const bool few = !given && plan.k <= THREADS / 2;
+        if (few) {
+            // the threads' largest tokens alone bound the k-th of all: what lies in
+            // their k-th's step or above is few
+            clear(sh);
+            if (hi > all.x) atomicAdd(&sh.hist[plan.step(hi)], 1ull);
             locate(sh, want_of);
-            const int bin = sh.bin;
-            if (bin < NB - 1) list.n = row.list(sh, [&](int i, float x) { return (plan.step(x) <= bin) & all.has(x, i); });
-        }
-        if (list.n > NB) {
-            kept = search(want_of, given);
-            list.n = row.list(sh, [&](int i, float x) { return kept.has(x, i); });
-            if (list.n <= NB) kept = all;
         } else {
+            search.divide(want_of, given);
+        }
+        const int bin = sh.bin;
+        const u64 above = sh.above;
+        const float low = plan.lowest(bin);
+        if (bin < NB - 1 && plan.k <= LIST) list.set(row.list(sh, [&](int, float x) { return x >= low; }));
+        if (list.fits()) {
             const Search<List, Step> among = {sh, list, plan.weigh, plan.step, true, all};
-            kept = among(want_of);
+            kept = few ? among(want_of) : among.within(bin, above, plan.k);
+        } else {
+            kept = few ? search(want_of) : bin < NB - 1 ? search.within(bin, above, plan.k) : all;
+            list.set(row.list(sh, [&](int i, float x) { return kept.has(x, i); }));
+            if (list.fits()) kept = all;
         }
     }
     if (plan.by_mass) {
         auto want_of = [&](u64 sum) { return share(plan.p, sum); };
-        if (list.n > NB) {
+        if (!list.fits()) {
             const Search<R, Step> search = {sh, row, plan.weigh, plan.step, false, kept};
             const u64 want = search.divide(want_of, plan.by_count ? nullptr : given);
             const int bin = sh.bin;
             const u64 above = sh.above;
             if (bin < NB - 1) {
-                list.n = row.list(sh, [&](int i, float x) { return (plan.step(x) <= bin) & kept.has(x, i); });
-                if (list.n <= NB) {
+                const float low = plan.lowest(bin);
+                if (plan.by_count)
+                    list.set(row.list(sh, [&](int i, float x) { return (x >= low) & kept.has(x, i); }));
+                else
+                    list.set(row.list(sh, [&](int, float x) { return x >= low; }));
+                if (list.fits()) {
                     const Search<List, Step> among = {sh, list, plan.weigh, plan.step, false, all};
                     kept = among.within(bin, above, want);
                 } else {
@@ -661,7 +714,7 @@ template <typename R>
 __device__ __forceinline__ float2 ends_of(Shared& sh, const R& row, float& hi) {
     float lo = INFINITY;
     hi = -INFINITY;
-    row.each([&](int, float x) {
+    row.template each<LIGHT>([&](int, float x) {
         hi = fmaxf(hi, x);  // NaN is passed over
         lo = fminf(lo, x > -INFINITY ? x : lo);
     });
@@ -671,7 +724,7 @@ template <typename R>
 __device__ __forceinline__ int first_of(Shared& sh, const R& row, float largest) {
     int first = 0x7fffffff;
     if (threadIdx.x == 0) sh.index = 0x7fffffff;
-    row.each([&](int i, float x) { first = min(first, x == largest ? i : 0x7fffffff); });
+    row.template each<LIGHT>([&](int i, float x) { first = min(first, x == largest ? i : 0x7fffffff); });
     __syncthreads();
     if (first != 0x7fffffff) atomicMin(&sh.index, first);
     __syncthreads();
@@ -692,9 +745,9 @@ __global__ void __launch_bounds__(THREADS) smg_sample_t(SampleArgs a) {
         found = first_of(sh, row, ends.y);
     } else if (ends.y > -INFINITY) {
         plan.init(sh, a, r, ends);
-        List list = {&sh, NB + 1};
+        List list = {&sh, NONE, 0};
         const Prefix kept = cut(sh, row, plan, list, hi, nullptr);
-        if (list.n <= NB)
+        if (list.fits())
             found = sh.list_i[plan.draw<true>(sh, list, kept)];
         else if (plan.by_count || plan.by_mass)
             found = plan.draw<true>(sh, row, kept);
@@ -771,9 +824,9 @@ __global__ void __launch_bounds__(THREADS) smg_sample_cut_t(SampleArgs a) {
         if (!plan.by_count && !plan.by_mass) {
             found = plan.draw<false>(sh, row, plan.all, w.blocks);
         } else {
-            List list = {&sh, NB + 1};
+            List list = {&sh, NONE, 0};
             const Prefix kept = cut(sh, row, plan, list, 0.f, w.hist);
-            open = list.n > NB;
+            open = !list.fits();
             if (open)
                 w.x = kept.x, w.i = kept.i;
             else
