@@ -295,9 +295,9 @@ struct Tile {
 
 // TREE: drafted nodes with their own K/V after the context.  KV8: e4m3 cache.
 // WR waves share the query rows of a tile (32 each), WK of them split its keys.
-template <bool TREE, bool KV8, int D, int WR>
+template <bool TREE, bool KV8, int D, int WR, int WK_>
 struct Shape {
-    static constexpr int WK = KV8 ? (WR == 8 ? 1 : 2) : 4 / WR;
+    static constexpr int WK = WK_;
     static constexpr int WAVES = WR * WK;
     static constexpr int THREADS = WAVES * WAVE;
     static constexpr int KB = WK == 1 ? 2 : 1;     // blocks of 32 keys a wave takes of a tile
@@ -307,14 +307,14 @@ struct Shape {
     static constexpr int RAW = TILE / 2;           // the same in 8 bits
     static constexpr int RAWS = 3;
     static constexpr int CHUNKS = 2 * TILE + (KV8 ? RAWS * RAW + (TREE ? TILE : 0) : 0);
-    static constexpr int SLOTS = KV8 || WR == 1 ? 256 : 512;  // workgroups that the card takes at once
+    static constexpr int SLOTS = KV8 || WK == 4 ? 256 : 512;  // workgroups that the card takes at once
     static constexpr int WAVES_A_SIMD = KV8 && WR == 2 ? 1 : WR == 1 ? 1 : 2;
 };
 
-template <bool TREE, bool KV8, int D, int WR>
-__global__ void __launch_bounds__((Shape<TREE, KV8, D, WR>::THREADS), (Shape<TREE, KV8, D, WR>::WAVES_A_SIMD)) smg_attn_cache_t(AttnArgs a) {
-    using Z = Shape<TREE, KV8, D, WR>;
-    constexpr int WK = Z::WK, KB = Z::KB, BN = Z::BN, BM = Z::BM, WAVES = Z::WAVES, THREADS = Z::THREADS;
+template <bool TREE, bool KV8, int D, int WR, int WK>
+__global__ void __launch_bounds__((Shape<TREE, KV8, D, WR, WK>::THREADS), (Shape<TREE, KV8, D, WR, WK>::WAVES_A_SIMD)) smg_attn_cache_t(AttnArgs a) {
+    using Z = Shape<TREE, KV8, D, WR, WK>;
+    constexpr int KB = Z::KB, BN = Z::BN, BM = Z::BM, WAVES = Z::WAVES, THREADS = Z::THREADS;
     constexpr int CPR = D / 8;               // 16-byte chunks a row
     constexpr int HB = D / 32;
     extern __shared__ u32x4 smem[];
@@ -718,12 +718,12 @@ __global__ void __launch_bounds__(256) smg_attn_join_t(AttnArgs a, int BM, int B
     *(bf16x4*)op = w;
 }
 
-template <bool TREE, bool KV8, int D, int WR>
+template <bool TREE, bool KV8, int D, int WR, int WK>
 int launch_t(AttnArgs a, hipStream_t s) {
-    using Z = Shape<TREE, KV8, D, WR>;
+    using Z = Shape<TREE, KV8, D, WR, WK>;
     constexpr int BM = Z::BM, BN = Z::BN;
     constexpr int tile_bytes = Z::CHUNKS * 16;
-    constexpr int join_bytes = Z::WK > 1 ? Z::WAVES * (D / 32 * 16 + 2) * WAVE * 4 : 0;
+    constexpr int join_bytes = WK > 1 ? Z::WAVES * (D / 32 * 16 + 2) * WAVE * 4 : 0;
     constexpr int bytes = tile_bytes > join_bytes ? tile_bytes : join_bytes;
     static_assert(bytes <= 160 * 1024, "LDS of a compute unit");
     const long long G = a.H / a.KVH;
@@ -737,12 +737,12 @@ int launch_t(AttnArgs a, hipStream_t s) {
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess) return -2;
     if (dev > 63 || !(set.load(std::memory_order_relaxed) >> dev & 1)) {
-        if (hipFuncSetAttribute((const void*)smg_attn_cache_t<TREE, KV8, D, WR>,
+        if (hipFuncSetAttribute((const void*)smg_attn_cache_t<TREE, KV8, D, WR, WK>,
                                 hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
             return -2;
         if (dev <= 63) set.fetch_or(1ull << dev, std::memory_order_relaxed);
     }
-    hipLaunchKernelGGL((smg_attn_cache_t<TREE, KV8, D, WR>), dim3((unsigned)grid), dim3(Z::THREADS), bytes, s, a);
+    hipLaunchKernelGGL((smg_attn_cache_t<TREE, KV8, D, WR, WK>), dim3((unsigned)grid), dim3(Z::THREADS), bytes, s, a);
     if (a.n_split > 1) {
         const long long rh = (TREE ? a.B * (long long)a.N : a.N) * a.H;
         if (rh > 0x7fffffffll) return -5;
@@ -752,22 +752,24 @@ int launch_t(AttnArgs a, hipStream_t s) {
 }
 
 template <bool TREE, bool KV8, int D>
-int launch_d(const AttnArgs& a, int wr, hipStream_t s) {
+int launch_d(const AttnArgs& a, int wr, int wk, hipStream_t s) {
     if constexpr (KV8) {
-        if (wr <= 2) return launch_t<TREE, true, D, 2>(a, s);
-        if (wr == 4) return launch_t<TREE, true, D, 4>(a, s);
-        return launch_t<TREE, true, D, 8>(a, s);
+        if (wr <= 2) return launch_t<TREE, true, D, 2, 2>(a, s);
+        if (wr == 4) return launch_t<TREE, true, D, 4, 2>(a, s);
+        return launch_t<TREE, true, D, 8, 1>(a, s);
     } else {
-        if constexpr (D == 128)
-            if (wr == 1) return launch_t<TREE, false, D, 1>(a, s);
-        if (wr <= 2) return launch_t<TREE, false, D, 2>(a, s);
-        return launch_t<TREE, false, D, 4>(a, s);
+        if constexpr (D == 128) {
+            if (wr == 1) return launch_t<TREE, false, D, 1, 4>(a, s);
+            if (wr == 2 && wk == 4) return launch_t<TREE, false, D, 2, 4>(a, s);
+        }
+        if (wr <= 2) return launch_t<TREE, false, D, 2, 2>(a, s);
+        return launch_t<TREE, false, D, 4, 1>(a, s);
     }
 }
 
 template <bool TREE, bool KV8>
-int launch(const AttnArgs& a, int D, int wr, hipStream_t s) {
-    return D == 128 ? launch_d<TREE, KV8, 128>(a, wr, s) : D == 64 ? launch_d<TREE, KV8, 64>(a, wr, s) : -1;
+int launch(const AttnArgs& a, int D, int wr, int wk, hipStream_t s) {
+    return D == 128 ? launch_d<TREE, KV8, 128>(a, wr, wk, s) : D == 64 ? launch_d<TREE, KV8, 64>(a, wr, wk, s) : -1;
 }
 
 int bad_shape(long long rows, int H, int KVH, int S, int T, int n_split) {
@@ -783,7 +785,7 @@ int bad_shape(long long rows, int H, int KVH, int S, int T, int n_split) {
 extern "C" int smg_attn_prefill_launch(
     const void* q, const void* k, const void* v, const void* slots, const void* ctx, const void* cu,
     void* out, void* part_o, void* part_ml, const long long* strides, int B, int N, int H, int KVH,
-    int S, int T, int D, int n_split, int wr, float scale, int kv_fp8, void* stream) {
+    int S, int T, int D, int n_split, int wr, int wk, float scale, int kv_fp8, void* stream) {
     if (int rc = bad_shape(N, H, KVH, S, T, n_split)) return rc;
     if (B < 1 || N < 1) return 0;
     AttnArgs a = {};
@@ -801,15 +803,15 @@ extern "C" int smg_attn_prefill_launch(
     a.v_ss = strides[7], a.v_sh = strides[8], a.v_st = strides[9];
     a.B = B, a.N = N, a.H = H, a.KVH = KVH, a.S = S, a.T = T, a.n_split = n_split;
     a.scale = scale;
-    return kv_fp8 ? launch<false, true>(a, D, wr, (hipStream_t)stream)
-                  : launch<false, false>(a, D, wr, (hipStream_t)stream);
+    return kv_fp8 ? launch<false, true>(a, D, wr, wk, (hipStream_t)stream)
+                  : launch<false, false>(a, D, wr, wk, (hipStream_t)stream);
 }
 
 // strides: q batch/token/head, out batch/token/head, k and v as above, k_new and v_new batch/token/head
 extern "C" int smg_attn_tree_launch(
     const void* q, const void* k_new, const void* v_new, const void* k, const void* v,
     const void* slots, const void* ctx, const void* parents, void* out, void* part_o, void* part_ml,
-    const long long* strides, int B, int N, int H, int KVH, int S, int T, int D, int n_split, int wr,
+    const long long* strides, int B, int N, int H, int KVH, int S, int T, int D, int n_split, int wr, int wk,
     float scale, int kv_fp8, void* stream) {
     if (int rc = bad_shape((long long)B * N, H, KVH, S, T, n_split)) return rc;
     if (N > 64) return -3;
@@ -834,6 +836,6 @@ extern "C" int smg_attn_tree_launch(
     a.vn_sb = strides[15], a.vn_st = strides[16], a.vn_sh = strides[17];
     a.B = B, a.N = N, a.H = H, a.KVH = KVH, a.S = S, a.T = T, a.n_split = n_split;
     a.scale = scale;
-    return kv_fp8 ? launch<true, true>(a, D, wr, (hipStream_t)stream)
-                  : launch<true, false>(a, D, wr, (hipStream_t)stream);
+    return kv_fp8 ? launch<true, true>(a, D, wr, wk, (hipStream_t)stream)
+                  : launch<true, false>(a, D, wr, wk, (hipStream_t)stream);
 }

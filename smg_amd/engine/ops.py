@@ -122,36 +122,38 @@ def _launch(kernel, dev: int, *args) -> None:
             kernel(*args, stream)
 
 
-def _shape(total: int, each: int, B: int, KVH: int, D: int, fp8: bool, ctx: int) -> Tuple[int, int]:
-    """How attention is cut: waves along the query rows of a workgroup (32 rows each), and
-    the most runs that a row's keys are split into (the kernel sizes them by the
-    sequences' lengths).  total: query rows of a kv head over all sequences, of which each
-    has `each`, or any number of them if that is 0.
+def _shape(total: int, each: int, B: int, KVH: int, D: int, fp8: bool, ctx: int) -> Tuple[int, int, int]:
+    """How attention is cut: waves of a workgroup along the query rows (32 each), waves along
+    the keys, and the most runs that a row's keys are split into (the kernel sizes them by
+    the sequences' lengths).  total: query rows of a kv head over all sequences, of which
+    each has `each`, or any number of them if that is 0.
 
     More rows a workgroup read K/V less often, but few workgroups leave compute units idle:
     the most rows that fill the card are taken (16 prompts of 70 tokens over 512 rows, 4 kv
-    heads: 21 us with 2 waves, 24 with 4, 37 with 1; 32 of them: 37, 32 and 63).  Splitting
-    keys fills it with few rows, and writes and reads partial results of as many rows as the
-    card takes at once: it has to save the time of about 1200 keys in 16 bits, 650 in 8
-    (one prompt of 256 tokens over 2000 rows: 29 us split, 31 not; over 500: 17 and 15)."""
+    heads: 21 us with 2 waves, 24 with 4, 37 with 1; 32 of them: 34, 32 and 63).  Where each
+    workgroup has a compute unit for itself, more waves take its keys (64 trees of 16 nodes
+    over 1400 rows: 38 us by 2 x 4 waves, 43 by 2 x 2; with twice the workgroups 43 and 34).
+    Splitting keys fills the card with few rows, and writes and reads partial results of as
+    many rows as it takes at once: it has to save the time of about 1450 keys in 16 bits,
+    650 in 8 (8 trees of 61 nodes over 2800 rows: 41 us split, 53 not; 16 prompts of 18
+    tokens over 2000: 33 and 29)."""
     def work(waves: int) -> int:
         at_once = 32 * waves
         return KVH * (B * -(-each // at_once) if each else max(B, total // at_once + B // 2))
 
-    wide = total > 128 * B  # sequences have more rows than 4 waves take
+    long = total > 128 * B and ctx >= 4096  # rows for 8 waves, and K/V worth reading once
     runs = max(1, min(64, ctx // 256))
     if fp8:
         four = work(4)
         if ctx * (256 - four) > 650 * 256:
-            return 8 if wide and ctx >= 4096 else 4, runs
-        return 8 if wide and work(8) >= 200 else 4 if four >= 100 else 2, 1
+            return (8, 1, runs) if long else (4, 2, runs)
+        return (8, 1, 1) if total > 128 * B and work(8) >= 200 else (4, 2, 1) if four >= 100 else (2, 2, 1)
     two = work(2)
-    fill = 512 if wide else 256  # two a compute unit, or one where K/V alone are the time
-    if ctx * (fill - two) > 1200 * fill:
-        return 4 if wide and ctx >= 4096 else 2, runs
-    if D == 128 and two <= 128:
-        return 1, 1
-    return 4 if total > 64 * B and work(4) >= 320 else 2, 1
+    if ctx * (256 - two) > 1450 * 256:
+        return (4, 1, runs) if long else (2, 2, runs)
+    if D == 128 and two <= 256:
+        return (1, 4, 1) if two <= 64 else (2, 4, 1)
+    return (4, 1, 1) if total > 64 * B and work(4) >= 320 else (2, 2, 1)
 
 
 def _parts(split: int, rows: int, D: int, q: torch.Tensor) -> tuple:
@@ -196,11 +198,11 @@ def attn_prefill(
         raise ValueError(f"at most {1 << 30} rows of a head, got {N} x {H}")
     total = N * (H // KVH)
     fp8 = k_cache.dtype is _FP8
-    wr, split = _shape(total, 0, B, KVH, D, fp8, T if max_ctx is None else min(int(max_ctx), T))
+    wr, wk, split = _shape(total, 0, B, KVH, D, fp8, T if max_ctx is None else min(int(max_ctx), T))
     part, po, pm = _parts(split, N * H, D, q)
     _launch(
         _core.attn_prefill, dev, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), p_slots, p_starts, p_cu,
-        out.data_ptr(), po, pm, strides, B, N, H, KVH, S, T, D, split, wr, scale, fp8,
+        out.data_ptr(), po, pm, strides, B, N, H, KVH, S, T, D, split, wr, wk, scale, fp8,
     )
     return out
 
@@ -244,11 +246,11 @@ def attn_tree(
         raise ValueError(f"at most {1 << 30} rows of a head, got {B} x {N} x {H}")
     rows = N * (H // KVH)
     fp8 = k_cache.dtype is _FP8
-    wr, split = _shape(B * rows, rows, B, KVH, D, fp8, T if max_ctx is None else min(int(max_ctx), T))
+    wr, wk, split = _shape(B * rows, rows, B, KVH, D, fp8, T if max_ctx is None else min(int(max_ctx), T))
     part, po, pm = _parts(split, B * N * H, D, q)
     _launch(
         _core.attn_tree, dev, q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-        p_slots, p_ctx, p_parents, out.data_ptr(), po, pm, strides, B, N, H, KVH, S, T, D, split, wr, scale, fp8,
+        p_slots, p_ctx, p_parents, out.data_ptr(), po, pm, strides, B, N, H, KVH, S, T, D, split, wr, wk, scale, fp8,
     )
     return out
 

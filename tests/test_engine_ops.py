@@ -385,6 +385,30 @@ def check_commit(args):
     return count
 
 
+# every way in which attention is cut, whatever the rule would take: waves along the rows
+# and along the keys, 8 bits
+SHAPES = [(1, 4, False), (2, 2, False), (2, 4, False), (4, 1, False), (2, 2, True), (4, 2, True), (8, 1, True)]
+
+
+@pytest.mark.gpu
+class TestAttnShapes:
+    @pytest.mark.parametrize("D", [64, 128])
+    @pytest.mark.parametrize("runs", [1, 5, 64])
+    @pytest.mark.parametrize("wr,wk,fp8", SHAPES)
+    def test_prefill(self, monkeypatch, wr, wk, fp8, runs, D):
+        monkeypatch.setattr(ops, "_shape", lambda *a: (wr, wk, runs))
+        args = prefill_case([1, 300, 0, 77, 130], [2100, 0, 50, 700, 3], 6, 2, D, fp8, seed=11)
+        check_prefill(ops.attn_prefill(*args), *args)
+
+    @pytest.mark.parametrize("D", [64, 128])
+    @pytest.mark.parametrize("runs", [1, 5, 64])
+    @pytest.mark.parametrize("wr,wk,fp8", SHAPES)
+    def test_tree(self, monkeypatch, wr, wk, fp8, runs, D):
+        monkeypatch.setattr(ops, "_shape", lambda *a: (wr, wk, runs))
+        args = tree_case(4, 39, [0, 1500, 64, 333], 6, 2, D, fp8, seed=12)
+        check_tree(ops.attn_tree(*args), *args)
+
+
 @pytest.mark.gpu
 class TestTreeCommit:
     @pytest.mark.parametrize("fp8", [False, True])
