@@ -17,15 +17,22 @@
 //
 // Both cuts are one search: the shortest prefix of the order whose measure (a
 // count, or a weight) reaches a number.  It runs over a histogram of NB equal
-// steps of the logit below the largest, which LDS atomics fill.  The tokens of
-// the step in which the number is reached are compared with each other; where
-// they are more than CAND, the step is divided again, until it holds few tokens
-// or one value, and equal values go by index.  Nothing is sorted.  What a cut
-// leaves is listed in index order if it fits, and all that follows runs over the
-// list.
+// steps of the logit below the largest, which LDS atomics fill (for a small top-k
+// each thread's largest token alone: they bound the k-th of all).  The tokens down to
+// the step in which the number is reached are listed in index order, if they fit,
+// and all that follows runs over the list.  The tokens of that step are compared with
+// each other; where they are more than CAND, the step is divided again, until it
+// holds few tokens or one value, and equal values go by index.  Nothing is sorted.
 //
 // A workgroup has a row, and each wave a run of it, 512 tokens at a time, 8 a
 // lane, so that index order is (wave, iteration, lane, element).
+//
+// What bounds it: a pass that weighs every token, about 45 vector instructions each, half
+// of them in 64 bits; without a cut that is one pass (512 rows of 32768 in bf16 on an
+// MI355X: 25 us, the memory's part 7), with a top-p one more that fills the histogram,
+// then the list (44 us), and where the list does not hold what is kept, a third.  A
+// top-k of 50 weighs only the list (19 us), temperature 0 none (10 us).  One row of
+// 2048: 2.3 us without a cut.
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>
 
