@@ -32,14 +32,14 @@
 //   16384 tokens, 16 over 4 heads of 128: 1.10 ms, 1.00 PF/s.  Matrix cores
 //     are busy 54% of the cycles and the vector unit, with exp and the
 //     roundings, 56%; under both the clock falls to 1.9 GHz.
-//   two chunks of 2000 tokens over 6000 8-bit rows, 16 heads: 273 us, 0.79 PF/s.
+//   two chunks of 1900 tokens over 5900 8-bit rows, 16 heads: 273 us, 0.79 PF/s.
 //     One workgroup of 8 waves a compute unit where 16 bits have two of 4, and
 //     7% for the widening.
-//   32 prompts of about 70 over 512 rows: 31 us; half of the units have two
+//   32 prompts of about 75 over 460 rows: 31 us; half of the units have two
 //     workgroups and the others one.
-//   64 trees of 16 nodes over 1400 rows: 51 us, 3.2 TB/s of K/V, 38 where the
-//     caches hold them: a tile's latency for each of 11 tiles in a row.
-//   4 trees of 61 over 33000 8-bit rows: 106 us, of which joining takes 9.
+//   64 trees of 16 nodes over 1150 rows: 51 us, 3.2 TB/s of K/V, 38 where the
+//     caches hold them: one tile's latency after the other.
+//   4 trees of 61 over 35000 8-bit rows: 106 us, of which joining takes 9.
 //   one prompt of a token, or a tree of 5: 6.5 and 7.5 us, latency alone.
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>

@@ -129,14 +129,14 @@ def _shape(total: int, each: int, B: int, KVH: int, D: int, fp8: bool, ctx: int)
     each has `each`, or any number of them if that is 0.
 
     More rows a workgroup read K/V less often, but few workgroups leave compute units idle:
-    the most rows that fill the card are taken (16 prompts of 70 tokens over 512 rows, 4 kv
+    the most rows that fill the card are taken (16 prompts of 75 tokens over 460 rows, 4 kv
     heads: 21 us with 2 waves, 24 with 4, 37 with 1; 32 of them: 34, 32 and 63).  Where each
     workgroup has a compute unit for itself, more waves take its keys (64 trees of 16 nodes
-    over 1400 rows: 38 us by 2 x 4 waves, 43 by 2 x 2; with twice the workgroups 43 and 34).
+    over 1150 rows: 38 us by 2 x 4 waves, 43 by 2 x 2; with twice the workgroups 43 and 34).
     Splitting keys fills the card with few rows, and writes and reads partial results of as
     many rows as it takes at once: it has to save the time of about 1450 keys in 16 bits,
-    650 in 8 (8 trees of 61 nodes over 2800 rows: 41 us split, 53 not; 16 prompts of 18
-    tokens over 2000: 33 and 29)."""
+    650 in 8 (8 trees of 61 nodes over up to 4000 rows: 41 us split, 53 not; 16 prompts of 18
+    tokens over up to 2000: 33 and 29)."""
     def work(waves: int) -> int:
         at_once = 32 * waves
         return KVH * (B * -(-each // at_once) if each else max(B, total // at_once + B // 2))
