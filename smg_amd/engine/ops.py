@@ -27,6 +27,7 @@ _CACHE_TYPES = (_BF16, _FP8)
 HEAD_DIMS = (64, 128)
 MAX_NODES = 64
 MAX_VOCAB = 1 << 20
+MAX_SEQUENCES = 1 << 16  # workgroups look through all sequences for their own
 
 try:
     from .. import _core
@@ -191,11 +192,11 @@ def attn_prefill(
     scale = _scale(scale, D)
     out = _out(out, q, dev)
     strides = _rows("q", q) + _rows("out", out) + cache_strides
+    if N * H > 1 << 30 or B > MAX_SEQUENCES:
+        raise ValueError(f"at most {1 << 30} rows of a head in {MAX_SEQUENCES} sequences, got {N} x {H} in {B}")
     _on_gpu("q", q, dev)
     if N == 0 or B == 0:
         return out
-    if N * H > 1 << 30:
-        raise ValueError(f"at most {1 << 30} rows of a head, got {N} x {H}")
     total = N * (H // KVH)
     fp8 = k_cache.dtype is _FP8
     wr, wk, split = _shape(total, 0, B, KVH, D, fp8, T if max_ctx is None else min(int(max_ctx), T))
@@ -239,11 +240,11 @@ def attn_tree(
     scale = _scale(scale, D)
     out = _out(out, q, dev)
     strides = _rows("q", q) + _rows("out", out) + cache_strides + _rows("k_new", k_new) + _rows("v_new", v_new)
+    if B * N * H > 1 << 30 or B > MAX_SEQUENCES:
+        raise ValueError(f"at most {1 << 30} rows of a head in {MAX_SEQUENCES} sequences, got {B} x {N} x {H}")
     _on_gpu("q", q, dev)
     if B == 0 or N == 0:
         return out
-    if B * N * H > 1 << 30:
-        raise ValueError(f"at most {1 << 30} rows of a head, got {B} x {N} x {H}")
     rows = N * (H // KVH)
     fp8 = k_cache.dtype is _FP8
     wr, wk, split = _shape(B * rows, rows, B, KVH, D, fp8, T if max_ctx is None else min(int(max_ctx), T))
@@ -283,6 +284,8 @@ def tree_commit(
         raise ValueError(f"kv_new {tuple(kv_new.shape)} does not fit kv_cache {tuple(kv_cache.shape)}")
     if D % 8:
         raise ValueError(f"head dim must be a multiple of 8, got {D}")
+    if B > MAX_SEQUENCES:
+        raise ValueError(f"at most {MAX_SEQUENCES} sequences, got {B}")
     if 0 in kv_cache.stride():
         raise ValueError(f"kv_cache must have a place for every element, strides {kv_cache.stride()}")
     if N > MAX_NODES or (N < 1 and B > 0):

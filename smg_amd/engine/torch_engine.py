@@ -846,7 +846,8 @@ class TorchEngine:
         if logits.dtype not in (torch.bfloat16, torch.float32):
             logits = logits.float()
         temperature, top_k, top_p, min_p = given
-        return ops.sample(logits, u, temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        # a row without a number (a broken model) answers with token 0
+        return ops.sample(logits, u, temperature, top_k=top_k, top_p=top_p, min_p=min_p).clamp_(min=0)
 
     # ---- forwards ----------------------------------------------------------
     def _kv_hist(self, li: int, which: int, slots):

@@ -652,6 +652,20 @@ class TestSample:
         u, t, p = torch.rand(20, generator=g, device=DEV), torch.ones(20, device=DEV), torch.full((20,), 0.9, device=DEV)
         replays(lambda: ops.sample(x, u, t, top_p=p), x)
 
+    def test_captured_with_shared_rows(self):
+        g = gen(10)
+        x = randn(g, 3, 70000, scale=2.0)
+        u, t, p = torch.rand(3, generator=g, device=DEV), torch.ones(3, device=DEV), torch.full((3,), 0.9, device=DEV)
+        replays(lambda: ops.sample(x, u, t, top_p=p), x)
+
+    @pytest.mark.parametrize("R,V", [(300, 3000), (2, 9000), (257, 9001)])
+    def test_threads_a_row(self, R, V):
+        # more rows than compute units, short rows, long ones
+        x = randn(gen(11), R, V, dtype=torch.float32, scale=2.0)
+        n = len(US)
+        check_sample(x, (US * R)[:R], [(0.0, 1.0, 0.7)[i % 3] for i in range(R)], k=[(0, 50, 1000, V)[i // n % 4] for i in range(R)],
+                     p=[(1.0, 0.9)[i % 2] for i in range(R)])
+
 
 class TestRefusals:
     """Refused on the host, before anything is launched: on CPU tensors."""
@@ -727,6 +741,14 @@ class TestRefusals:
         ("commit", dict(tokens=torch.zeros(2, 3, dtype=torch.int32)), TypeError),
         ("commit", dict(targets=torch.zeros(3, 2, dtype=torch.int64)), ValueError),
         ("prefill", dict(out=torch.zeros(1, 4, 64, dtype=BF16).expand(6, 4, 64)), ValueError),
+        ("prefill", dict(slots=torch.zeros(65537, dtype=torch.int32), starts=torch.zeros(65537, dtype=torch.int32),
+                         cu=torch.zeros(65538, dtype=torch.int32)), ValueError),
+        ("tree", dict(q=torch.zeros(1, 1, 4, 64, dtype=BF16).expand(65537, 1, 4, 64), kn=torch.zeros(1, 1, 2, 64, dtype=BF16).expand(65537, 1, 2, 64),
+                      vn=torch.zeros(1, 1, 2, 64, dtype=BF16).expand(65537, 1, 2, 64), slots=torch.zeros(65537, dtype=torch.int32),
+                      ctx=torch.zeros(65537, dtype=torch.int32), parents=torch.zeros(65537, 1, dtype=torch.int32)), ValueError),
+        ("commit", dict(kn=torch.zeros(1, 2, 1, 1, 2, 64, dtype=BF16).expand(1, 2, 65537, 1, 2, 64), slots=torch.zeros(65537, dtype=torch.int32),
+                        ctx=torch.zeros(65537, dtype=torch.int32), parents=torch.zeros(65537, 1, dtype=torch.int32),
+                        tokens=torch.zeros(65537, 1, dtype=torch.int64), targets=torch.zeros(65537, 1, dtype=torch.int64)), ValueError),
         ("commit", dict(kv=torch.zeros(1, 2, 1, 2, 16, 64, dtype=BF16).expand(1, 2, 4, 2, 16, 64)), ValueError),
         ("prefill", dict(q=torch.zeros(6, 4, 64, dtype=BF16, requires_grad=True)), RuntimeError),
         ("tree", dict(q=torch.zeros(2, 3, 4, 64, dtype=BF16, requires_grad=True)), RuntimeError),
