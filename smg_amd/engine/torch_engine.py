@@ -60,7 +60,8 @@ class TorchEngineConfig:
     kv_fp8: bool = False
     # opt-in packed prefill: prompts and chunks of different lengths and
     # histories share one forward (ops.attn_prefill) instead of waiting for
-    # others of their length.  Requires the gfx950 kernels.
+    # others of their length (32 prompts of 40 to 400 tokens: 22 ms, 224
+    # without).  Requires the gfx950 kernels.
     packed_prefill: bool = False
 
     @classmethod
@@ -1326,7 +1327,8 @@ class TorchEngine:
     def _prefill_packed(self, items: List[tuple]) -> torch.Tensor:
         """Prefill of `items` = [(slot, start, tokens)] of any lengths and histories in
         one forward over their packed tokens; returns the sampled tokens ([len(items)],
-        device)."""
+        device).  Over an 8-bit cache a chunk reads its own tokens in 8 bits too, as
+        decoding does, where _prefill_batch reads them in 16."""
         c = self.cfg
         lens = np.asarray([len(toks) for _, _, toks in items], dtype=np.int64)
         slots_np = np.asarray([s for s, _, _ in items], dtype=np.int64)
