@@ -41,7 +41,6 @@
 #define WAVE 64
 #define NB 2048             // steps of a histogram; also the most blocks
 #define BLOCK 512           // tokens of a wave's iteration
-#define CAND 128            // tokens that are compared with each other
 #define MAX_V (NB * BLOCK)
 #define DEEP 2              // loads of a wave on their way in a pass that computes
 #define LIGHT 4             // and in one that only compares
@@ -114,8 +113,9 @@ __device__ __forceinline__ u64 at_lane(u64 x, int lane) {
 }
 __device__ __forceinline__ u64 wave_sum(u64 x) { return at_lane(wave_scan(x), 63); }
 
-// What a workgroup of THREADS does, with up to LIST listed tokens.
-template <int THREADS, int LIST>
+// What a workgroup of THREADS does, with up to LIST listed tokens, and CAND that are
+// compared with each other.
+template <int THREADS, int LIST, int CAND = 128>
 struct Sampler {
     static constexpr int WAVES = THREADS / WAVE;
 
@@ -772,7 +772,9 @@ __global__ void __launch_bounds__(THREADS) smg_sample_t(SampleArgs a) {
 // Each of the passes over a row that cost the most (the largest logit, the first cut's
 // measures, the last sums) has `parts` workgroups a row; the searches between them have
 // one.  Integer sums make the answer the same.
-using Wide = Sampler<1024, 8192>;
+// Their steps hold more tokens: 64 rows of 131071 take 71 us where 256 are compared, 82 with
+// 128 and another division; 512 shorter rows 58 and 56.
+using Wide = Sampler<1024, 8192, 256>;
 using Slim = Sampler<1024, 1024>;  // where nothing is listed: more workgroups fit a compute unit
 __device__ __forceinline__ float2 ends_of(const Work& w, int parts) {
     const int lane = threadIdx.x & 63;

@@ -308,9 +308,9 @@ def tree_commit(
 
 def _parts_of(R: int, V: int) -> int:
     """Workgroups that share a row of logits: few long rows leave most of the card idle.
-    One row of 131072 alone and shared by 8: 69 and 42 us with a top-p, 39 and 14 without a
-    cut, 26 and 30 with a top-k of 50; 64 rows alone and by 4, of mixed settings: 118 and
-    83.  Below 65536 the five launches cost what they save."""
+    One row of 131072 alone and shared by 8: 69 and 44 us with a top-p, 39 and 14 without a
+    cut, 26 and 30 with a top-k of 50; 64 rows alone and by 4, of mixed settings: 117 and
+    70.  Below 65536 the five launches cost what they save."""
     if V < 65536 or R > 128:
         return 1
     return max(1, min(16, V // 16384, 256 // R))
