@@ -29,10 +29,10 @@
 //
 // What bounds it: a pass that weighs every token, about 45 vector instructions each, half
 // of them in 64 bits; without a cut that is one pass (512 rows of 32768 in bf16 on an
-// MI355X: 25 us, the memory's part 7), with a top-p one more that fills the histogram,
-// then the list (44 us), and where the list does not hold what is kept, a third.  A
-// top-k of 50 weighs only the list (19 us), temperature 0 none (10 us).  One row of
-// 2048: 2.3 us without a cut.
+// MI355X: 25 us, the memory's part 7), with a top-p the one that fills the histogram, and
+// the list after it (44 us), or another pass where the list does not hold what is kept
+// (61 us).  A top-k of 50 weighs only the list (19 us), temperature 0 nothing (10 us).
+// One row of 2048 with a top-p: 8.2 us, most of it barriers and latency.
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>
 
