@@ -793,9 +793,9 @@ class TorchEngine:
 
     def _h2d_i64(self, arr) -> torch.Tensor:
         """Small int64 host->device transfer that does NOT block the host:
-        pinned staging + non_blocking copy into a persistent device buffer
-        (rotating 12-deep so in-flight DMAs are never overwritten within the
-        pipeline's one-tick lag)."""
+        pinned staging + non_blocking copy into a persistent device buffer,
+        rotating 12-deep.  A long burst behind a busy stream comes round to a
+        buffer whose copy has not run yet: its event is waited for first."""
         arr = np.ascontiguousarray(arr, dtype=np.int64)
         n = arr.shape[0]
         if self.device.type != "cuda":
@@ -805,11 +805,15 @@ class TorchEngine:
         if entry is None or entry[0].numel() < n:
             cap = max(n, 3 * (self.cfg.max_slots + 8))
             entry = (torch.empty(cap, dtype=torch.long, pin_memory=True),
-                     torch.empty(cap, dtype=torch.long, device=self.device))
+                     torch.empty(cap, dtype=torch.long, device=self.device),
+                     torch.cuda.Event())
             self._h2d_bufs[self._h2d_i] = entry
-        pin, dev = entry
+        else:
+            entry[2].synchronize()
+        pin, dev, copied = entry
         pin[:n].numpy()[:] = arr
         dev[:n].copy_(pin[:n], non_blocking=True)
+        copied.record()
         return dev[:n]
 
     def _get_slab(self, n: int) -> torch.Tensor:

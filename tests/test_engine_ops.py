@@ -1025,3 +1025,57 @@ class TestEnginePaths:
             got = eng.step_drafts({r: ([3, 4], [-1, -1]) for r in rids})
             eng.step()  # and decoding goes on in between
             assert all(got.values())
+
+
+class TestStaging:
+    def test_a_buffer_is_not_written_before_its_copy_ran(self, monkeypatch):
+        """The ring of transfers on the CPU, with copies that run only when they are waited for."""
+        stream, ran = [], []  # sources of the copies that have not run, values of those that have
+
+        def run(n):
+            ran.extend(src.tolist() for src in stream[:n])
+            del stream[:n]
+
+        class Event:
+            def record(self):
+                self.place = len(ran) + len(stream)
+
+            def synchronize(self):
+                run(max(0, self.place - len(ran)))
+
+        class Device(torch.Tensor):
+            def copy_(self, src, non_blocking=False):
+                stream.append(src)
+                return self
+
+        empty = torch.empty
+
+        def cpu_empty(*a, pin_memory=False, device=None, **kw):
+            t = empty(*a, **kw)
+            return t if device is None else t.as_subclass(Device)
+
+        eng = engine("cpu")
+        eng.device = torch.device(DEV)
+        monkeypatch.setattr(torch, "empty", cpu_empty)
+        monkeypatch.setattr(torch.cuda, "Event", Event)
+        sent = [[i] * (1 + i % 5) for i in range(3 * len(eng._h2d_bufs))]
+        for values in sent:
+            eng._h2d_i64(values)
+        assert stream  # the host ran ahead
+        run(len(stream))
+        assert ran == sent
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("packed", [False, True])
+    def test_a_long_burst_behind_a_busy_stream(self, packed):
+        outs = []
+        for busy in (False, True):
+            eng = engine(packed_prefill=packed, max_slots=8)
+            rids = [eng.submit([(i * 37 + j) % 2048 for j in range(20 + i)], 40 + i) for i in range(6)]
+            for _ in range(8):
+                if busy:
+                    torch.cuda._sleep(20_000_000)  # some milliseconds: the host is far ahead
+                eng.step(decode_burst=16)
+            assert all(eng.finished(r) for r in rids)
+            outs.append([eng.collect(r) for r in rids])
+        assert outs[0] == outs[1]
