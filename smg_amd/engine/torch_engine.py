@@ -149,8 +149,9 @@ GREEDY = (0.0, 0, 1.0, 0.0)  # (temperature, top_k, top_p, min_p)
 def _sampling_of(temperature, top_k, top_p, min_p) -> tuple:
     """A request's sampling settings, checked; GREEDY for temperature 0."""
     s = (float(temperature), max(0, int(top_k)), float(top_p), float(min_p))
-    if not (0 <= s[0] < math.inf and 0 < s[2] <= 1 and 0 <= s[3] <= 1 and s[1] < 2 ** 31):
-        raise ValueError(f"sampling needs a temperature >= 0, an int32 top_k, 0 < top_p <= 1 and 0 <= min_p <= 1, got {s}")
+    # the slots hold them in 32 bits
+    if not (0 <= s[0] <= torch.finfo(torch.float32).max and 0 < s[2] <= 1 and 0 <= s[3] <= 1 and s[1] < 2 ** 31):
+        raise ValueError(f"sampling needs a float32 temperature >= 0, an int32 top_k, 0 < top_p <= 1 and 0 <= min_p <= 1, got {s}")
     return s if s[0] > 0 else GREEDY
 
 
@@ -831,9 +832,9 @@ class TorchEngine:
     # ---- sampling ----------------------------------------------------------
     def _set_sampling(self, slot: int, sampling: tuple) -> None:
         if self._sampling_host[slot] != sampling:
-            self._sampling_host[slot] = sampling
             for t, v in zip(self._sampling, sampling):
                 t[slot] = v
+            self._sampling_host[slot] = sampling
 
     def _samples(self) -> bool:
         """Whether a running request samples: all greedy, the forwards end in an argmax."""

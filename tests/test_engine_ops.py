@@ -872,6 +872,21 @@ class TestEngineSampling:
             with pytest.raises(ValueError):
                 eng.submit([1, 2], 2, **kw)
 
+    def test_a_temperature_beyond_float32_is_refused_before_anything_is_taken(self):
+        eng = engine("cpu")
+        most = torch.finfo(torch.float32).max
+        for t in (1e39, most * (1 + 2.0 ** -24), 10 ** 300):
+            with pytest.raises(ValueError, match="float32"):
+                eng.submit([1, 2], 2, temperature=t)
+            with pytest.raises(ValueError, match="float32"):
+                eng.import_kv("x", torch.zeros(eng.kv_transfer_shape(3)), 3, 1, 4, temperature=t)
+        assert not eng.waiting and not eng.running and len(eng._free_slots) == eng.cfg.max_slots
+        rids = [eng.submit([1, 2], 3, temperature=t) for t in (most, 1e-46, 0.5)]
+        assert all(len(out) == 3 for out in run(eng, *rids))
+        # what the slots hold on the device is what the host takes them to hold
+        for slot, s in enumerate(eng._sampling_host):
+            assert [t[slot].item() for t in eng._sampling] == torch.tensor(s, dtype=torch.float32).tolist()
+
     def test_settings_follow_the_kv(self):
         a, b = engine("cpu"), engine("cpu")
         rid = a.submit(list(range(30)), 8, prefill_only=True, temperature=2.0)
