@@ -72,14 +72,16 @@ struct AttnArgs {
     const int* ctx;              // [B] rows in the cache before the new tokens
     const int* cu;               // prefill: [B + 1] first packed row of each sequence
     const int* parents;          // tree: [B, N]
-    float* part_o;               // n_split > 1: [n_split, rows, H, D], unnormalised
-    float* part_ml;              // n_split > 1: [n_split, rows, H, 2]
+    float* part_o;               // n_split > 1: [units, KVH, part_rows, D], unnormalised
+    float* part_ml;              // n_split > 1: [units, KVH, part_rows, 2]
     long long q_sb, q_st, q_sh, o_sb, o_st, o_sh;        // strides in elements
     long long k_ss, k_sh, k_st, v_ss, v_sh, v_st;
     long long kn_sb, kn_st, kn_sh, vn_sb, vn_st, vn_sh;
     int B, N, H, KVH, S, T;
     int n_split;                 // most runs that a row's keys are split into
     int share;                   // workgroups that the card takes at once, for each kv head
+    int units;                   // of a kv head: tiles of rows, or with n_split > 1 their runs at most
+    int part_rows;               // of a tile: BM, or all there are if fewer
     float scale;
 };
 
@@ -115,13 +117,15 @@ struct Seq {
 // side.  A run is as long as the tiles of all rows over the workgroups that the card
 // takes at once (less one for each tile of rows, whose last run is a part): then long
 // sequences have many runs and short ones one, which writes its result itself.  Every
-// wave of both kernels computes the same.
-__device__ __forceinline__ int run_length(const AttnArgs& a, int BM, int BN, bool tree) {
+// wave of both kernels computes the same.  mine: a lane's (row tiles, key tiles) of its
+// sequence among the first 64.
+__device__ __forceinline__ int run_length(const AttnArgs& a, int BM, int BN, bool tree, int2* mine = nullptr) {
     if (a.n_split == 1) return 0x7fffffff;
     const int lane = threadIdx.x & 63, G = a.H / a.KVH;
     float tiles = 0.f, rows = 0.f;
     for (int b = lane; b < a.B; b += WAVE) {
         const Seq s(a, b, G, BM, BN, tree);
+        if (mine && b == lane) *mine = make_int2(s.row_tiles, s.key_tiles);
         tiles += (float)s.row_tiles * (float)s.key_tiles;
         rows += (float)s.row_tiles;
     }
@@ -134,6 +138,11 @@ __device__ __forceinline__ int run_length(const AttnArgs& a, int BM, int BN, boo
 // tiles of a run in a sequence whose last tile of rows has `most` key tiles
 __device__ __forceinline__ int run_of(const AttnArgs& a, int most, int length) {
     return max(1, max(min(length, most), (most + a.n_split - 1) / a.n_split));
+}
+// and the runs that each of its tiles of rows has
+__device__ __forceinline__ int runs_of(const AttnArgs& a, int most, int length) {
+    const int per = run_of(a, most, length);
+    return max(1, (most + per - 1) / per);
 }
 
 // max and sum over the two halves of a wave (lane and lane ^ 32)
@@ -363,8 +372,7 @@ __global__ void __launch_bounds__((Shape<TREE, KV8, D, WR, WK>::THREADS), (Shape
             if (b0 + lane < a.B) {
                 const Seq s(a, b0 + lane, G, BM, BN, TREE);
                 first = s.base, all = s.rows;
-                const int per = run_of(a, s.key_tiles, length);
-                runs = max(1, (s.key_tiles + per - 1) / per);
+                runs = runs_of(a, s.key_tiles, length);
                 n = s.row_tiles * runs;
             }
             int sum = n;
@@ -631,8 +639,10 @@ __global__ void __launch_bounds__((Shape<TREE, KV8, D, WR, WK>::THREADS), (Shape
     if (!live) return;
     const int hb0 = WK > 1 ? wk * HW : 0;
     if (runs > 1) {
-        const size_t all_rows = (size_t)(TREE ? a.B * (long long)a.N : a.N);
-        const size_t at = ((size_t)split * all_rows + (TREE ? (size_t)b * a.N : base) + token) * a.H + head;
+        // by workgroup: the runs that there are at most are far more than those that
+        // the card takes
+        const int unit = gridDim.x / a.KVH - 1 - blockIdx.x / a.KVH;
+        const size_t at = ((size_t)unit * a.KVH + kvh) * a.part_rows + wr * 32 + col;
 #pragma unroll
         for (int hb = 0; hb < HW; ++hb)
 #pragma unroll
@@ -670,11 +680,9 @@ __global__ void __launch_bounds__(256) smg_attn_join_t(AttnArgs a, int BM, int B
     if (rh >= all_rows * a.H) return;
     const long long r = rh / a.H;
     const int h = (int)(rh % a.H), G = a.H / a.KVH;
-    int b, rows, token;
+    int b;
     if constexpr (TREE) {
         b = (int)(r / a.N);
-        token = (int)(r % a.N);
-        rows = a.N * G;
     } else {
         // the last sequence that starts at r or before; rows outside all stay
         if (r < a.cu[0] || r >= a.cu[a.B]) return;
@@ -687,25 +695,33 @@ __global__ void __launch_bounds__(256) smg_attn_join_t(AttnArgs a, int BM, int B
                 hi = mid;
         }
         b = lo;
-        const int first = max(a.cu[b], 0);
-        token = (int)r - first;
-        rows = (min(a.cu[b + 1], a.N) - first) * G;
     }
-    const int slot = a.slots[b];
-    if (slot < 0 || slot >= a.S) return;
-    const int last_row = min((token * G + h % G) / BM * BM + BM, rows) - 1;
-    const int ctx = context(a, b, TREE);
-    const int kend = keys_of(a, ctx, last_row, G, TREE);
-    const int new_tiles = TREE ? (a.N + BN - 1) / BN : 0;
-    const int most = (keys_of(a, ctx, rows - 1, G, TREE) + BN - 1) / BN + new_tiles;
-    const int per = run_of(a, most, run_length(a, BM, BN, TREE));
-    const int n = ((kend + BN - 1) / BN + new_tiles + per - 1) / per;
+    const Seq seq(a, b, G, BM, BN, TREE);
+    const int token = TREE ? (int)(r % a.N) : (int)r - seq.base;
+    const int row = token * G + h % G, tile = row / BM;
+    if (!seq.key_tiles || row >= seq.rows) return;
+    const int last_row = min(tile * BM + BM, seq.rows) - 1;
+    const int kend = keys_of(a, context(a, b, TREE), last_row, G, TREE);
+    int2 mine = make_int2(0, 0);
+    const int length = run_length(a, BM, BN, TREE, &mine);
+    const int per = run_of(a, seq.key_tiles, length);
+    const int n = ((kend + BN - 1) / BN + (TREE ? (a.N + BN - 1) / BN : 0) + per - 1) / per;
     if (n <= 1) return;
+    // the workgroups before this tile's, as the other kernel counts them
+    int before = lane < b ? mine.x * runs_of(a, mine.y, length) : 0;
+    for (int i = lane + WAVE; i < b; i += WAVE) {
+        const Seq s(a, i, G, BM, BN, TREE);
+        before += s.row_tiles * runs_of(a, s.key_tiles, length);
+    }
+#pragma unroll
+    for (int o = 1; o < WAVE; o <<= 1) before += __shfl_xor(before, o, WAVE);
+    const int first = before + tile * runs_of(a, seq.key_tiles, length);
+    if (first < 0 || first > a.units - n) return;  // offsets that do not rise
     // a lane a run (at most 64 of them)
     const float c = a.scale * LOG2E;
-    const size_t run = all_rows * a.H;
+    const size_t run = (size_t)a.KVH * a.part_rows, at = (size_t)first * run + (size_t)(h / G) * a.part_rows + row % BM;
     float ms = -INFINITY, ls = 0.f;
-    if (lane < n) ms = a.part_ml[(lane * run + rh) * 2], ls = a.part_ml[(lane * run + rh) * 2 + 1];
+    if (lane < n) ms = a.part_ml[(lane * run + at) * 2], ls = a.part_ml[(lane * run + at) * 2 + 1];
     float top = ms;
 #pragma unroll
     for (int o = 1; o < WAVE; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, WAVE));
@@ -721,7 +737,7 @@ __global__ void __launch_bounds__(256) smg_attn_join_t(AttnArgs a, int BM, int B
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const int s = s0 + i * RPL + lane / LPR;
-            part[i] = s < n ? *(const f32x4*)(a.part_o + (s * run + rh) * D + e) : (f32x4)0.f;
+            part[i] = s < n ? *(const f32x4*)(a.part_o + (s * run + at) * D + e) : (f32x4)0.f;
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) o += __shfl(fs, s0 + i * RPL + lane / LPR, WAVE) * part[i];
@@ -739,8 +755,9 @@ __global__ void __launch_bounds__(256) smg_attn_join_t(AttnArgs a, int BM, int B
     *(bf16x4*)op = w;
 }
 
+// `floats`, if given, gets the size of the workspace instead of a launch
 template <bool TREE, bool KV8, int D, int WR, int WK>
-int launch_t(AttnArgs a, hipStream_t s) {
+int launch_t(AttnArgs a, hipStream_t s, long long* floats) {
     using Z = Shape<TREE, KV8, D, WR, WK>;
     constexpr int BM = Z::BM, BN = Z::BN;
     constexpr int tile_bytes = Z::CHUNKS * 16;
@@ -750,9 +767,19 @@ int launch_t(AttnArgs a, hipStream_t s) {
     const long long G = a.H / a.KVH;
     const long long tiles = TREE ? a.B * ((a.N * G + BM - 1) / BM) : a.N * G / BM + a.B;
     // with runs: never more than `share` of them, but at least one for each tile of rows
-    a.share = (int)(Z::SLOTS / a.KVH > tiles ? Z::SLOTS / a.KVH : tiles);
-    const long long grid = (a.n_split > 1 ? a.share : tiles) * a.KVH;
-    if (grid > 0x7fffffffll || a.n_split > WAVE) return -5;
+    const long long share = Z::SLOTS / a.KVH > tiles ? Z::SLOTS / a.KVH : tiles;
+    const long long units = share < tiles * a.n_split ? share : tiles * a.n_split;
+    const long long grid = units * a.KVH;
+    if (grid > 0x7fffffffll || share > 0x7fffffffll || a.n_split > WAVE) return -5;
+    a.part_rows = (int)(a.N * G < BM ? a.N * G : BM);
+    if (floats) {
+        *floats = a.n_split > 1 ? grid * a.part_rows * (D + 2) : 0;
+        return 0;
+    }
+    if (a.n_split > 1 && !a.part_o) return -3;
+    a.share = (int)share;
+    a.units = (int)units;
+    a.part_ml = a.part_o + grid * a.part_rows * D;
     // more dynamic LDS than the default limit, once a device
     static std::atomic<unsigned long long> set{0};
     int dev = 0;
@@ -773,24 +800,24 @@ int launch_t(AttnArgs a, hipStream_t s) {
 }
 
 template <bool TREE, bool KV8, int D>
-int launch_d(const AttnArgs& a, int wr, int wk, hipStream_t s) {
+int launch_d(const AttnArgs& a, int wr, int wk, hipStream_t s, long long* floats) {
     if constexpr (KV8) {
-        if (wr <= 2) return launch_t<TREE, true, D, 2, 2>(a, s);
-        if (wr == 4) return launch_t<TREE, true, D, 4, 2>(a, s);
-        return launch_t<TREE, true, D, 8, 1>(a, s);
+        if (wr <= 2) return launch_t<TREE, true, D, 2, 2>(a, s, floats);
+        if (wr == 4) return launch_t<TREE, true, D, 4, 2>(a, s, floats);
+        return launch_t<TREE, true, D, 8, 1>(a, s, floats);
     } else {
         if constexpr (D == 128) {
-            if (wr == 1) return launch_t<TREE, false, D, 1, 4>(a, s);
-            if (wr == 2 && wk == 4) return launch_t<TREE, false, D, 2, 4>(a, s);
+            if (wr == 1) return launch_t<TREE, false, D, 1, 4>(a, s, floats);
+            if (wr == 2 && wk == 4) return launch_t<TREE, false, D, 2, 4>(a, s, floats);
         }
-        if (wr <= 2) return launch_t<TREE, false, D, 2, 2>(a, s);
-        return launch_t<TREE, false, D, 4, 1>(a, s);
+        if (wr <= 2) return launch_t<TREE, false, D, 2, 2>(a, s, floats);
+        return launch_t<TREE, false, D, 4, 1>(a, s, floats);
     }
 }
 
 template <bool TREE, bool KV8>
-int launch(const AttnArgs& a, int D, int wr, int wk, hipStream_t s) {
-    return D == 128 ? launch_d<TREE, KV8, 128>(a, wr, wk, s) : D == 64 ? launch_d<TREE, KV8, 64>(a, wr, wk, s) : -1;
+int launch(const AttnArgs& a, int D, int wr, int wk, hipStream_t s, long long* floats) {
+    return D == 128 ? launch_d<TREE, KV8, 128>(a, wr, wk, s, floats) : D == 64 ? launch_d<TREE, KV8, 64>(a, wr, wk, s, floats) : -1;
 }
 
 int bad_shape(long long rows, int H, int KVH, int S, int T, int n_split) {
@@ -802,10 +829,21 @@ int bad_shape(long long rows, int H, int KVH, int S, int T, int n_split) {
 
 }  // namespace
 
+// floats of workspace that a call with n_split > 1 takes, or an error below 0
+extern "C" long long smg_attn_part_floats(int tree, int B, int N, int H, int KVH, int D, int n_split, int wr, int wk, int kv_fp8) {
+    if (int rc = bad_shape(tree ? (long long)B * N : N, H, KVH, 1, 1, n_split)) return rc;
+    AttnArgs a = {};
+    a.B = B, a.N = N, a.H = H, a.KVH = KVH, a.n_split = n_split;
+    long long floats = 0;
+    const int rc = tree ? kv_fp8 ? launch<true, true>(a, D, wr, wk, nullptr, &floats) : launch<true, false>(a, D, wr, wk, nullptr, &floats)
+                        : kv_fp8 ? launch<false, true>(a, D, wr, wk, nullptr, &floats) : launch<false, false>(a, D, wr, wk, nullptr, &floats);
+    return rc ? rc : floats;
+}
+
 // strides: q token/head, out token/head, k slot/head/row, v slot/head/row
 extern "C" int smg_attn_prefill_launch(
     const void* q, const void* k, const void* v, const void* slots, const void* ctx, const void* cu,
-    void* out, void* part_o, void* part_ml, const long long* strides, int B, int N, int H, int KVH,
+    void* out, void* part, const long long* strides, int B, int N, int H, int KVH,
     int S, int T, int D, int n_split, int wr, int wk, float scale, int kv_fp8, void* stream) {
     if (int rc = bad_shape(N, H, KVH, S, T, n_split)) return rc;
     if (B < 1 || N < 1) return 0;
@@ -817,21 +855,20 @@ extern "C" int smg_attn_prefill_launch(
     a.slots = (const int*)slots;
     a.ctx = (const int*)ctx;
     a.cu = (const int*)cu;
-    a.part_o = (float*)part_o;
-    a.part_ml = (float*)part_ml;
+    a.part_o = (float*)part;
     a.q_st = strides[0], a.q_sh = strides[1], a.o_st = strides[2], a.o_sh = strides[3];
     a.k_ss = strides[4], a.k_sh = strides[5], a.k_st = strides[6];
     a.v_ss = strides[7], a.v_sh = strides[8], a.v_st = strides[9];
     a.B = B, a.N = N, a.H = H, a.KVH = KVH, a.S = S, a.T = T, a.n_split = n_split;
     a.scale = scale;
-    return kv_fp8 ? launch<false, true>(a, D, wr, wk, (hipStream_t)stream)
-                  : launch<false, false>(a, D, wr, wk, (hipStream_t)stream);
+    return kv_fp8 ? launch<false, true>(a, D, wr, wk, (hipStream_t)stream, nullptr)
+                  : launch<false, false>(a, D, wr, wk, (hipStream_t)stream, nullptr);
 }
 
 // strides: q batch/token/head, out batch/token/head, k and v as above, k_new and v_new batch/token/head
 extern "C" int smg_attn_tree_launch(
     const void* q, const void* k_new, const void* v_new, const void* k, const void* v,
-    const void* slots, const void* ctx, const void* parents, void* out, void* part_o, void* part_ml,
+    const void* slots, const void* ctx, const void* parents, void* out, void* part,
     const long long* strides, int B, int N, int H, int KVH, int S, int T, int D, int n_split, int wr, int wk,
     float scale, int kv_fp8, void* stream) {
     if (int rc = bad_shape((long long)B * N, H, KVH, S, T, n_split)) return rc;
@@ -847,8 +884,7 @@ extern "C" int smg_attn_tree_launch(
     a.slots = (const int*)slots;
     a.ctx = (const int*)ctx;
     a.parents = (const int*)parents;
-    a.part_o = (float*)part_o;
-    a.part_ml = (float*)part_ml;
+    a.part_o = (float*)part;
     a.q_sb = strides[0], a.q_st = strides[1], a.q_sh = strides[2];
     a.o_sb = strides[3], a.o_st = strides[4], a.o_sh = strides[5];
     a.k_ss = strides[6], a.k_sh = strides[7], a.k_st = strides[8];
@@ -857,6 +893,6 @@ extern "C" int smg_attn_tree_launch(
     a.vn_sb = strides[15], a.vn_st = strides[16], a.vn_sh = strides[17];
     a.B = B, a.N = N, a.H = H, a.KVH = KVH, a.S = S, a.T = T, a.n_split = n_split;
     a.scale = scale;
-    return kv_fp8 ? launch<true, true>(a, D, wr, wk, (hipStream_t)stream)
-                  : launch<true, false>(a, D, wr, wk, (hipStream_t)stream);
+    return kv_fp8 ? launch<true, true>(a, D, wr, wk, (hipStream_t)stream, nullptr)
+                  : launch<true, false>(a, D, wr, wk, (hipStream_t)stream, nullptr);
 }

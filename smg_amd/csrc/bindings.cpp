@@ -80,14 +80,15 @@ int smg_attn_decode_launch_ex(const void* q, const void* k, const void* v, const
                               float scale, void* stream, int kv_fp8);
 // ---- attention of many new tokens over the slot cache (attn_cache.hip) ----
 int smg_attn_prefill_launch(const void* q, const void* k, const void* v, const void* slots,
-                            const void* ctx, const void* cu, void* out, void* part_o,
-                            void* part_ml, const long long* strides, int B, int N, int H, int KVH,
+                            const void* ctx, const void* cu, void* out, void* part,
+                            const long long* strides, int B, int N, int H, int KVH,
                             int S, int T, int D, int n_split, int wr, int wk, float scale,
                             int kv_fp8, void* stream);
 int smg_attn_tree_launch(const void* q, const void* k_new, const void* v_new, const void* k,
                          const void* v, const void* slots, const void* ctx, const void* parents,
-                         void* out, void* part_o, void* part_ml, const long long* strides, int B,
+                         void* out, void* part, const long long* strides, int B,
                          int N, int H, int KVH, int S, int T, int D, int n_split, int wr, int wk, float scale, int kv_fp8, void* stream);
+long long smg_attn_part_floats(int tree, int B, int N, int H, int KVH, int D, int n_split, int wr, int wk, int kv_fp8);
 // ---- drafted tokens into the cache (tree_commit.hip) ----
 int smg_tree_commit_launch(const void* src, void* dst, const void* slots, const void* ctx,
                            const void* parents, const void* tokens, const void* targets,
@@ -508,41 +509,49 @@ PYBIND11_MODULE(_core, m) {
     // smg_amd/engine/ops.py checks the tensors and sizes the split
     m.def("attn_prefill",
           [](uintptr_t q, uintptr_t k, uintptr_t v, uintptr_t slots, uintptr_t ctx, uintptr_t cu,
-             uintptr_t out, uintptr_t part_o, uintptr_t part_ml, std::vector<long long> strides,
+             uintptr_t out, uintptr_t part, std::vector<long long> strides,
              int B, int N, int H, int KVH, int S, int T, int D, int n_split, int wr, int wk,
              float scale, int kv_fp8, uintptr_t stream) {
               if (strides.size() != 10) throw std::runtime_error("attn_prefill takes 10 strides");
               int rc = smg_attn_prefill_launch(
                   (const void*)q, (const void*)k, (const void*)v, (const void*)slots,
-                  (const void*)ctx, (const void*)cu, (void*)out, (void*)part_o, (void*)part_ml,
+                  (const void*)ctx, (const void*)cu, (void*)out, (void*)part,
                   strides.data(), B, N, H, KVH, S, T, D, n_split, wr, wk, scale, kv_fp8,
                   (void*)stream);
               if (rc != 0) throw std::runtime_error("attn_prefill launch failed rc=" + std::to_string(rc));
           },
           py::arg("q"), py::arg("k"), py::arg("v"), py::arg("slots"), py::arg("ctx"),
-          py::arg("cu"), py::arg("out"), py::arg("part_o"), py::arg("part_ml"), py::arg("strides"),
+          py::arg("cu"), py::arg("out"), py::arg("part"), py::arg("strides"),
           py::arg("B"), py::arg("N"), py::arg("H"), py::arg("KVH"), py::arg("S"), py::arg("T"),
           py::arg("D"), py::arg("n_split"), py::arg("wr"), py::arg("wk"), py::arg("scale"),
           py::arg("kv_fp8"), py::arg("stream"));
     m.def("attn_tree",
           [](uintptr_t q, uintptr_t k_new, uintptr_t v_new, uintptr_t k, uintptr_t v,
-             uintptr_t slots, uintptr_t ctx, uintptr_t parents, uintptr_t out, uintptr_t part_o,
-             uintptr_t part_ml, std::vector<long long> strides, int B, int N, int H, int KVH, int S,
+             uintptr_t slots, uintptr_t ctx, uintptr_t parents, uintptr_t out, uintptr_t part,
+             std::vector<long long> strides, int B, int N, int H, int KVH, int S,
              int T, int D, int n_split, int wr, int wk, float scale, int kv_fp8,
              uintptr_t stream) {
               if (strides.size() != 18) throw std::runtime_error("attn_tree takes 18 strides");
               int rc = smg_attn_tree_launch(
                   (const void*)q, (const void*)k_new, (const void*)v_new, (const void*)k,
                   (const void*)v, (const void*)slots, (const void*)ctx, (const void*)parents,
-                  (void*)out, (void*)part_o, (void*)part_ml, strides.data(), B, N, H, KVH, S, T, D,
+                  (void*)out, (void*)part, strides.data(), B, N, H, KVH, S, T, D,
                   n_split, wr, wk, scale, kv_fp8, (void*)stream);
               if (rc != 0) throw std::runtime_error("attn_tree launch failed rc=" + std::to_string(rc));
           },
           py::arg("q"), py::arg("k_new"), py::arg("v_new"), py::arg("k"), py::arg("v"),
-          py::arg("slots"), py::arg("ctx"), py::arg("parents"), py::arg("out"), py::arg("part_o"),
-          py::arg("part_ml"), py::arg("strides"), py::arg("B"), py::arg("N"), py::arg("H"),
+          py::arg("slots"), py::arg("ctx"), py::arg("parents"), py::arg("out"), py::arg("part"),
+          py::arg("strides"), py::arg("B"), py::arg("N"), py::arg("H"),
           py::arg("KVH"), py::arg("S"), py::arg("T"), py::arg("D"), py::arg("n_split"),
           py::arg("wr"), py::arg("wk"), py::arg("scale"), py::arg("kv_fp8"), py::arg("stream"));
+    m.def("attn_part_floats",
+          [](bool tree, int B, int N, int H, int KVH, int D, int n_split, int wr, int wk, bool kv_fp8) {
+              const long long n = smg_attn_part_floats(tree, B, N, H, KVH, D, n_split, wr, wk, kv_fp8);
+              if (n < 0) throw std::runtime_error("attn_part_floats failed rc=" + std::to_string(n));
+              return n;
+          },
+          py::arg("tree"), py::arg("B"), py::arg("N"), py::arg("H"), py::arg("KVH"), py::arg("D"),
+          py::arg("n_split"), py::arg("wr"), py::arg("wk"), py::arg("kv_fp8"));
     // accepted drafts into the cache (tree_commit.hip)
     m.def("tree_commit",
           [](uintptr_t src, uintptr_t dst, uintptr_t slots, uintptr_t ctx, uintptr_t parents,

@@ -157,12 +157,12 @@ def _shape(total: int, each: int, B: int, KVH: int, D: int, fp8: bool, ctx: int)
     return (4, 1, 1) if total > 64 * B and work(4) >= 320 else (2, 2, 1)
 
 
-def _parts(split: int, rows: int, D: int, q: torch.Tensor) -> tuple:
-    """Workspace of the splits' partial results: the tensor, and the addresses of its halves."""
+def _parts(q: torch.Tensor, tree: bool, B: int, N: int, H: int, KVH: int, D: int, split: int, wr: int, wk: int, fp8: bool):
+    """Workspace of the runs' partial results: a place for every row of the workgroups that
+    the card takes at once, 17 or 34 MB at a head dim of 128, however many runs a row may have."""
     if split == 1:
-        return None, 0, 0
-    part = torch.empty(split * rows * (D + 2), dtype=_F32, device=q.device)
-    return part, part.data_ptr(), part.data_ptr() + split * rows * D * 4
+        return None
+    return torch.empty(_core.attn_part_floats(tree, B, N, H, KVH, D, split, wr, wk, fp8), dtype=_F32, device=q.device)
 
 
 def attn_prefill(
@@ -200,10 +200,10 @@ def attn_prefill(
     total = N * (H // KVH)
     fp8 = k_cache.dtype is _FP8
     wr, wk, split = _shape(total, 0, B, KVH, D, fp8, T if max_ctx is None else min(int(max_ctx), T))
-    part, po, pm = _parts(split, N * H, D, q)
+    part = _parts(q, False, B, N, H, KVH, D, split, wr, wk, fp8)
     _launch(
         _core.attn_prefill, dev, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), p_slots, p_starts, p_cu,
-        out.data_ptr(), po, pm, strides, B, N, H, KVH, S, T, D, split, wr, wk, scale, fp8,
+        out.data_ptr(), 0 if part is None else part.data_ptr(), strides, B, N, H, KVH, S, T, D, split, wr, wk, scale, fp8,
     )
     return out
 
@@ -248,10 +248,10 @@ def attn_tree(
     rows = N * (H // KVH)
     fp8 = k_cache.dtype is _FP8
     wr, wk, split = _shape(B * rows, rows, B, KVH, D, fp8, T if max_ctx is None else min(int(max_ctx), T))
-    part, po, pm = _parts(split, B * N * H, D, q)
+    part = _parts(q, True, B, N, H, KVH, D, split, wr, wk, fp8)
     _launch(
         _core.attn_tree, dev, q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-        p_slots, p_ctx, p_parents, out.data_ptr(), po, pm, strides, B, N, H, KVH, S, T, D, split, wr, wk, scale, fp8,
+        p_slots, p_ctx, p_parents, out.data_ptr(), 0 if part is None else part.data_ptr(), strides, B, N, H, KVH, S, T, D, split, wr, wk, scale, fp8,
     )
     return out
 

@@ -409,6 +409,55 @@ class TestAttnShapes:
         check_tree(ops.attn_tree(*args), *args)
 
 
+class TestWorkspace:
+    @pytest.mark.parametrize("N,H,KVH,T,fp8,most", [
+        (2000, 16, 16, 131072, True, 256 * 256), (1000, 16, 16, 65536, False, 512 * 128), (900, 16, 4, 65536, False, 512 * 128),
+        (1, 8, 2, 1 << 20, True, 64 * 8),
+    ])
+    def test_size_goes_by_what_the_card_takes(self, monkeypatch, N, H, KVH, T, fp8, most):
+        """At most `most` rows of partial results, each of 128 values and its maximum and sum."""
+        sizes = []
+        monkeypatch.setattr(ops, "_on_gpu", lambda *a: None)
+        monkeypatch.setattr(ops, "_launch", lambda *a: None)
+        empty = torch.empty
+        monkeypatch.setattr(torch, "empty", lambda *a, **k: sizes.append(a[0]) or empty(0))
+        cache = torch.zeros(1, 1, 1, 128, dtype=FP8 if fp8 else BF16).expand(1, KVH, T, 128)
+        one, new = torch.zeros(1, dtype=torch.int32), min(N, 64)
+        ops.attn_prefill(torch.zeros(N, H, 128, dtype=BF16), cache, cache, one, one, torch.tensor([0, N], dtype=torch.int32))
+        kn = torch.zeros(1, new, KVH, 128, dtype=BF16)
+        ops.attn_tree(torch.zeros(1, new, H, 128, dtype=BF16), kn, kn, cache, cache, one, one, torch.zeros(1, new, dtype=torch.int32))
+        assert len(sizes) == 2 and 0 < max(sizes) <= most * 130
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("wr,wk,fp8", SHAPES)
+    def test_calls_stay_in_it(self, monkeypatch, wr, wk, fp8):
+        held = []
+
+        def parts(q, *shape):
+            n = ops._core.attn_part_floats(*shape)
+            held.append(torch.full((n + 2048,), 7.0, device=DEV))
+            return held[-1][1024:-1024]
+
+        monkeypatch.setattr(ops, "_shape", lambda *a: (wr, wk, 64))
+        monkeypatch.setattr(ops, "_parts", parts)
+        # more sequences than lanes, some of them empty or padding, few of them long
+        lens = [(i * 7) % 23 for i in range(150)]
+        args = prefill_case(lens, [(3000 if i % 40 == 39 else i) for i in range(150)], 8, 4, 128, fp8, seed=2)
+        args[3][70] = -1
+        out = ops.attn_prefill(*args, out=torch.zeros_like(args[0]))
+        cu = args[5].tolist()
+        assert (out[cu[70]:cu[71]] == 0).all()
+        for b in (39, 64, 69, 71, 79, 149):
+            part = [args[0][cu[b]:cu[b + 1]], args[1], args[2], args[3][b:b + 1], args[4][b:b + 1], i32([0, lens[b]])]
+            check_prefill(out[cu[b]:cu[b + 1]], *part)
+        args = tree_case(70, 9, [(4000 if i % 33 == 32 else i) for i in range(70)], 4, 2, 128, fp8, seed=3)
+        out = ops.attn_tree(*args)
+        pick = [0, 32, 63, 64, 65, 69]
+        check_tree(out[pick], *(t[pick] for t in args[:3]), *args[3:5], *(t[pick] for t in args[5:]))
+        for t in held:
+            assert (t[:1024] == 7).all() and (t[-1024:] == 7).all() and (t[1024:-1024] != 7).any()
+
+
 @pytest.mark.gpu
 class TestTreeCommit:
     @pytest.mark.parametrize("fp8", [False, True])
