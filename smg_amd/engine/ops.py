@@ -9,8 +9,9 @@ bfloat16 or float8_e4m3fn; its dimensions may have any strides but the last,
 which is dense.  Rows of tensors that kernels read 16 bytes at a time start at
 multiples of 16 bytes (8 where tree_commit writes an 8-bit cache).
 
-They are forwards without a gradient, for a worker that answers: a first argument
-that asks for one is refused where gradients are recorded.
+They are forwards without a gradient, for a worker that answers: any argument that
+asks for one is refused where gradients are recorded, and one with a forward-mode
+tangent always.
 
 What the host cannot see is bounded on the device: a sequence whose slot lies
 outside the cache is a padding entry, lengths and offsets are cut to the tensors.
@@ -21,6 +22,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 _BF16, _FP8, _I32, _I64, _F32 = (torch.bfloat16, torch.float8_e4m3fn, torch.int32, torch.int64, torch.float32)
 _CACHE_TYPES = (_BF16, _FP8)
@@ -104,10 +106,19 @@ def _out(out: Optional[torch.Tensor], q: torch.Tensor, dev: int) -> torch.Tensor
     return out
 
 
-def _on_gpu(name: str, t: torch.Tensor, dev: int) -> None:
-    if t.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError(f"{name} asks for a gradient, and the operators have none: detach it or use torch.no_grad()")
+def _on_gpu(dev: int, **floats) -> None:
+    """That the call can run: floats are its arguments that could ask for a gradient, the
+    first argument first."""
+    if torch.is_grad_enabled():
+        for name, t in floats.items():
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{name} asks for a gradient, and the operators have none: detach it or use torch.no_grad()")
+    if forward_ad._current_level >= 0:
+        for name, t in floats.items():
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{name} has a tangent, and the operators have none: take its primal")
     if dev < 0:
+        name, t = next(iter(floats.items()))
         raise RuntimeError(f"{name} is on {t.device}: the operators run on a CUDA/HIP device")
     if _core is None:
         raise RuntimeError("smg_amd._core (gfx950 kernels) is not built: run `python -m smg_amd.csrc.build`")
@@ -194,7 +205,7 @@ def attn_prefill(
     strides = _rows("q", q) + _rows("out", out) + cache_strides
     if N * H > 1 << 30 or B > MAX_SEQUENCES:
         raise ValueError(f"at most {1 << 30} rows of a head in {MAX_SEQUENCES} sequences, got {N} x {H} in {B}")
-    _on_gpu("q", q, dev)
+    _on_gpu(dev, q=q, k_cache=k_cache, v_cache=v_cache, out=out)
     if N == 0 or B == 0:
         return out
     total = N * (H // KVH)
@@ -242,7 +253,7 @@ def attn_tree(
     strides = _rows("q", q) + _rows("out", out) + cache_strides + _rows("k_new", k_new) + _rows("v_new", v_new)
     if B * N * H > 1 << 30 or B > MAX_SEQUENCES:
         raise ValueError(f"at most {1 << 30} rows of a head in {MAX_SEQUENCES} sequences, got {B} x {N} x {H}")
-    _on_gpu("q", q, dev)
+    _on_gpu(dev, q=q, k_new=k_new, v_new=v_new, k_cache=k_cache, v_cache=v_cache, out=out)
     if B == 0 or N == 0:
         return out
     rows = N * (H // KVH)
@@ -296,7 +307,7 @@ def tree_commit(
         _index("parents", parents, (B, N), dev), _index("tokens", tokens, (B, N), dev, _I64),
         _index("targets", targets, (B, N), dev, _I64),
     )
-    _on_gpu("kv_new", kv_new, dev)
+    _on_gpu(dev, kv_new=kv_new, kv_cache=kv_cache)
     count, path, nxt = torch.empty_like(ctx_lens), torch.empty_like(parents), tokens.new_empty(B)
     if B:
         _launch(
@@ -351,7 +362,7 @@ def sample(
     p_m = 0 if min_p is None else _index("min_p", min_p, rows, dev, _F32)
     if out is not None:
         _index("out", out, rows, dev, _I64)
-    _on_gpu("logits", logits, dev)
+    _on_gpu(dev, logits=logits, u=u, temperature=temperature, top_p=top_p, min_p=min_p)
     if out is None:
         out = torch.empty(rows, dtype=_I64, device=logits.device)
     if R:

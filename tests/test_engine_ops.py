@@ -820,6 +820,27 @@ class TestRefusals:
             getattr(self, call)(**kw)
 
 
+    @pytest.mark.parametrize("call,name,shape,dtype", [
+        ("prefill", "q", (6, 4, 64), BF16), ("prefill", "k", (2, 2, 16, 64), BF16), ("prefill", "v", (2, 2, 16, 64), BF16),
+        ("prefill", "out", (6, 4, 64), BF16), ("tree", "q", (2, 3, 4, 64), BF16), ("tree", "kn", (2, 3, 2, 64), BF16),
+        ("tree", "vn", (2, 3, 2, 64), BF16), ("tree", "k", (2, 2, 16, 64), BF16), ("tree", "v", (2, 2, 16, 64), BF16),
+        ("commit", "kn", (1, 2, 2, 3, 2, 64), BF16), ("commit", "kv", (1, 2, 4, 2, 16, 64), BF16),
+        ("sample", "logits", (2, 9), torch.float32), ("sample", "u", (2,), torch.float32),
+        ("sample", "temperature", (2,), torch.float32), ("sample", "top_p", (2,), torch.float32), ("sample", "min_p", (2,), torch.float32),
+    ])
+    def test_gradients_are_refused_for_every_argument(self, call, name, shape, dtype):
+        x = torch.ones(shape, dtype=dtype)
+        with pytest.raises(RuntimeError, match="gradient"):
+            getattr(self, call)(**{name: x.clone().requires_grad_()})
+        with torch.autograd.forward_ad.dual_level():
+            dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+            with pytest.raises(RuntimeError, match="tangent"):
+                getattr(self, call)(**{name: dual})
+        # and neither where there is none
+        with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA/HIP"):
+            getattr(self, call)(**{name: x.clone().requires_grad_()})
+
+
 @pytest.mark.gpu
 class TestTogether:
     def test_empty_batches(self):
