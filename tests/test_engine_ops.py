@@ -417,8 +417,8 @@ class TestWorkspace:
     def test_size_goes_by_what_the_card_takes(self, monkeypatch, N, H, KVH, T, fp8, most):
         """At most `most` rows of partial results, each of 128 values and its maximum and sum."""
         sizes = []
-        monkeypatch.setattr(ops, "_on_gpu", lambda *a: None)
-        monkeypatch.setattr(ops, "_launch", lambda *a: None)
+        monkeypatch.setattr(ops, "_on_gpu", lambda *a, **k: None)
+        monkeypatch.setattr(ops, "_launch", lambda *a, **k: None)
         empty = torch.empty
         monkeypatch.setattr(torch, "empty", lambda *a, **k: sizes.append(a[0]) or empty(0))
         cache = torch.zeros(1, 1, 1, 128, dtype=FP8 if fp8 else BF16).expand(1, KVH, T, 128)
