@@ -33,8 +33,11 @@ MAX_SEQUENCES = 1 << 16  # workgroups look through all sequences for their own
 
 try:
     from .. import _core
-except ImportError:  # refusals work without the built core; _launch says that it is missing
+except ImportError:  # refusals work without the built core
     _core = None
+# a core built from older sources may lack these kernels
+BUILT = all(hasattr(_core, k) for k in ("attn_prefill", "attn_tree", "attn_part_floats", "tree_commit", "sample", "sample_work_bytes"))
+NOT_BUILT = "smg_amd._core lacks the gfx950 kernels of smg_amd.engine.ops: run `python -m smg_amd.csrc.build`"
 
 
 # The checks are written for speed: one condition a tensor, and the reasons only
@@ -120,8 +123,8 @@ def _on_gpu(dev: int, **floats) -> None:
     if dev < 0:
         name, t = next(iter(floats.items()))
         raise RuntimeError(f"{name} is on {t.device}: the operators run on a CUDA/HIP device")
-    if _core is None:
-        raise RuntimeError("smg_amd._core (gfx950 kernels) is not built: run `python -m smg_amd.csrc.build`")
+    if not BUILT:
+        raise RuntimeError(NOT_BUILT)
 
 
 def _launch(kernel, dev: int, *args) -> None:

@@ -393,7 +393,7 @@ class TorchEngine:
 
     def _has_ops(self) -> bool:
         """Whether attention over the cache runs on the kernels of ops.py."""
-        return (self._hip_fused is not None and getattr(self, "_hip_rope_prefill", None) is not None
+        return (ops.BUILT and self._hip_fused is not None and getattr(self, "_hip_rope_prefill", None) is not None
                 and self.cfg.head_dim in ops.HEAD_DIMS)
 
     # ---- API -------------------------------------------------------------
@@ -416,7 +416,7 @@ class TorchEngine:
         `temperature` above 0 samples the request's tokens (ops.sample) with
         `top_k` (0: all), `top_p` (1: all) and `min_p` (0: none) from the
         engine's own generator; 0 takes the likeliest token."""
-        sampling = _sampling_of(temperature, top_k, top_p, min_p)
+        sampling = self._sampling_settings(temperature, top_k, top_p, min_p)
         if rid is None:
             self._rid_counter += 1
             rid = f"req-{self._rid_counter}"
@@ -485,7 +485,7 @@ class TorchEngine:
         """Decode-leg intake: place the transferred KV into a free slot and
         continue decoding from the prefill-sampled first token, with the
         sampling settings of submit()."""
-        sampling = _sampling_of(temperature, top_k, top_p, min_p)
+        sampling = self._sampling_settings(temperature, top_k, top_p, min_p)
         if not self._free_slots:
             return False
         c = self.cfg
@@ -830,6 +830,12 @@ class TorchEngine:
         return s
 
     # ---- sampling ----------------------------------------------------------
+    def _sampling_settings(self, temperature, top_k, top_p, min_p) -> tuple:
+        s = _sampling_of(temperature, top_k, top_p, min_p)
+        if s[0] > 0 and self.device.type == "cuda" and not ops.BUILT:
+            raise RuntimeError(ops.NOT_BUILT)  # here, not in the middle of a step
+        return s
+
     def _set_sampling(self, slot: int, sampling: tuple) -> None:
         if self._sampling_host[slot] != sampling:
             for t, v in zip(self._sampling, sampling):

@@ -977,6 +977,36 @@ class TestEngineSampling:
             eng.step_drafts({})
 
 
+    def test_a_core_without_the_kernels_is_found_out_before_a_step(self, monkeypatch):
+        eng = engine("cpu")
+        eng._hip_fused = eng._hip_rope_prefill = object()  # as a core from older sources has them
+        assert eng._has_ops()
+        monkeypatch.setattr(ops, "BUILT", False)
+        assert not eng._has_ops()
+        with pytest.raises(RuntimeError, match="step_drafts"):
+            eng.step_drafts({})
+        eng.device = torch.device(DEV)
+        kv = torch.zeros(eng.kv_transfer_shape(3))
+        for call in (lambda **kw: eng.submit([1, 2], 2, **kw), lambda **kw: eng.import_kv("x", kv, 3, 1, 4, **kw)):
+            with pytest.raises(RuntimeError, match="csrc.build"):
+                call(temperature=0.5)
+        assert not eng.waiting and len(eng._free_slots) == eng.cfg.max_slots
+        eng.submit([1, 2], 2)  # greedy ones do without
+
+    def test_kernels_are_looked_for_by_name(self, monkeypatch):
+        import importlib
+
+        from smg_amd import _core
+
+        try:
+            assert ops.BUILT
+            monkeypatch.delattr(_core, "tree_commit")
+            assert not importlib.reload(ops).BUILT
+        finally:
+            monkeypatch.undo()
+            assert importlib.reload(ops).BUILT
+
+
 def kv_rows(eng, slot, n):
     return eng.kv[:, :, slot, :, :n].float()
 
