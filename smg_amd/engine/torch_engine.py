@@ -644,8 +644,8 @@ class TorchEngine:
         if pending:
             pending.sort(key=lambda sr: len(sr[1].tokens) - sr[1].prefilled)
         if pending and c.packed_prefill:
-            # the shortest first, each as far as the tokens of a forward go
-            group, lens, room = [], [], int(c.prefill_budget_mult * c.prefill_chunk)
+            # the shortest first, each as far as the tokens of a forward go: a chunk at least
+            group, lens, room = [], [], int(max(1.0, c.prefill_budget_mult) * c.prefill_chunk)
             for slot, req in pending[: c.prefill_group]:
                 n = min(len(req.tokens) - req.prefilled, c.prefill_chunk, room)
                 if n <= 0:

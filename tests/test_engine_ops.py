@@ -1011,6 +1011,25 @@ def kv_rows(eng, slot, n):
     return eng.kv[:, :, slot, :, :n].float()
 
 
+@pytest.mark.parametrize("mult", [0.0, 1e-3, 0.4, 1.0, 2.5])
+def test_packed_groups_follow_the_budget(monkeypatch, mult):
+    """A forward takes the budget's tokens, and a chunk where that is less: all prompts end."""
+    eng = engine("cpu", prefill_chunk=16, prefill_budget_mult=mult, prefix_cache_slots=0)
+    eng.cfg.packed_prefill = True  # with the batched forward in the kernels' place
+    taken = []
+
+    def packed(items):
+        taken.append([len(toks) for _, _, toks in items])
+        return torch.cat([eng._prefill_batch([item]) for item in items])
+
+    monkeypatch.setattr(eng, "_prefill_packed", packed)
+    prompts = [list(range(n)) for n in (3, 40, 16, 17, 1)]
+    got = run(eng, *[eng.submit(p, 3) for p in prompts])
+    ref = engine("cpu", prefix_cache_slots=0)
+    assert got == run(ref, *[ref.submit(p, 3) for p in prompts])
+    assert all(0 < sum(lens) <= max(16, 16 * mult) and max(lens) <= 16 for lens in taken)
+
+
 @pytest.mark.gpu
 class TestEnginePaths:
     @pytest.mark.parametrize("kw", [{}, dict(n_kv_heads=2), dict(n_kv_heads=2, kv_fp8=True), dict(prefill_chunk=24, prefill_budget_mult=1.0)])
