@@ -1213,3 +1213,144 @@ class TestStaging:
             assert all(eng.finished(r) for r in rids)
             outs.append([eng.collect(r) for r in rids])
         assert outs[0] == outs[1]
+
+
+SD = 12 * HALF * math.sqrt(1 / 3)
+"""How far a logit of the tiny engine may be off between two ways to compute it, as a
+standard deviation.  Two layers of six roundings to bf16 each, were all of them half a step
+in one direction, leave the last state off by 12 HALF of its length, sqrt(d).  A logit is
+its product with a row of the embedding, whose direction has nothing to do with it and whose
+length is sqrt(1/3): uniform numbers of up to 1/sqrt(d) in size.  8-bit K/V add half a step
+of theirs, 2^-4 of what attention adds, in both layers."""
+SD_FP8 = SD + 2 * 2.0 ** -4 * math.sqrt(1 / 3)
+
+
+def watch(eng):
+    """The logits of every choice that the engine makes from now on."""
+    seen, choose = [], eng._choose
+
+    def keep(logits, *a, **kw):
+        seen.append(logits.float())
+        return choose(logits, *a, **kw)
+
+    eng._choose = keep
+    return seen
+
+
+def lead(logits):
+    """By how much the likeliest token leads."""
+    two = logits.topk(2, dim=-1).values
+    return two[..., 0] - two[..., 1]
+
+
+@pytest.mark.gpu
+class TestEngineAnswers:
+    """What the engine's ways through the operators answer, against its other ways."""
+
+    @pytest.mark.parametrize("kw", [{}, dict(n_kv_heads=1), dict(n_kv_heads=2, kv_fp8=True)])
+    def test_packed_prefill_answers_as_the_batched_one(self, kw):
+        sd = SD_FP8 if kw.get("kv_fp8") else SD
+        g = torch.Generator().manual_seed(1)
+        prompts = [torch.randint(0, 2048, (n,), generator=g).tolist() for n in (5, 130, 1, 64, 97, 33, 200)]
+        # 530 tokens, in one forward (4 chunks of 256)
+        plain, packed = engine(prefix_cache_slots=0, **kw), engine(prefix_cache_slots=0, packed_prefill=True, prefill_budget_mult=4.0, **kw)
+        want, got = [], watch(packed)
+        for p in prompts:
+            seen = watch(plain)
+            plain.submit(p, 1)
+            plain.step()
+            want.append(seen[0][0])
+        state, prefill = [], packed._prefill_packed
+
+        def kept(items):
+            nxt = prefill(items)
+            state.append((items, nxt.tolist(), packed._last_tok.tolist(), packed.seq_len.tolist()))
+            return nxt
+
+        packed._prefill_packed = kept
+        rids = [packed.submit(p, 9) for p in prompts]
+        packed.step()
+        (items, nxt, last, lens), = state
+        assert len(items) == len(prompts)
+        by_slot = {packed._requests[r].slot: i for i, r in enumerate(rids)}
+        for row, ((slot, start, _), token) in enumerate(zip(items, nxt)):
+            i = by_slot[slot]
+            # 2048 logits of a few prompts stay below 6 deviations, and are rounded to bf16 twice
+            assert (got[0][row] - want[i]).abs().max() <= 6 * sd + 2 * HALF * want[i].abs().max()
+            assert token == got[0][row].argmax().item() == last[slot] == packed._requests[rids[i]].generated[0]
+            assert start == 0 and lens[slot] == len(prompts[i])
+
+    @pytest.mark.parametrize("kw", [{}, dict(n_kv_heads=2), dict(n_kv_heads=2, kv_fp8=True)])
+    def test_drafted_steps_choose_as_decoding_does(self, kw):
+        sd = SD_FP8 if kw.get("kv_fp8") else SD
+        decoded, drafted = engine(max_slots=32, vocab_size=32, **kw), engine(max_slots=32, vocab_size=32, **kw)
+        g = torch.Generator().manual_seed(2)
+        prompts = [torch.randint(0, 32, (11 + i,), generator=g).tolist() for i in range(24)]
+        rids = [[e.submit(p, 60) for p in prompts] for e in (decoded, drafted)]
+        for e, rr in zip((decoded, drafted), rids):
+            while any(not e._requests[r].generated for r in rr):
+                e.step()
+        # both chose their first tokens, and the ones of the steps so far, in the same way
+        assert all(decoded._requests[a].generated == drafted._requests[b].generated for a, b in zip(*rids))
+        seen, compared, clear = watch(decoded), 0, dict.fromkeys(range(len(prompts)), True)
+        for _ in range(10):
+            decoded.step()
+            got = drafted.step_drafts({r: ([1], [-1]) for r in rids[1]})
+            logits = seen[-1]
+            for i, ok in clear.items():
+                req = decoded._requests[rids[0][i]]
+                # one that leads by less may lose: the requests' texts part from there on
+                clear[i] = ok = ok and lead(logits[req.slot]).item() > 4 * math.sqrt(2) * sd and len(got[rids[1][i]]) == 1
+                if ok:
+                    assert got[rids[1][i]][0] == req.generated[-1]
+                    compared += 1
+        assert compared >= (8 if kw.get("kv_fp8") else 20)
+
+    @pytest.mark.parametrize("settings", [{}, dict(temperature=1.5, top_k=1)])
+    @pytest.mark.parametrize("kw", [{}, dict(n_kv_heads=2), dict(n_kv_heads=2, kv_fp8=True)])
+    def test_a_chain_of_right_drafts_lies_in_the_cache_as_its_prefill(self, kw, settings):
+        one, eng = engine(max_slots=64, vocab_size=32, **kw), engine(max_slots=64, vocab_size=32, **kw)
+        g = torch.Generator().manual_seed(3)
+        prompts = [torch.randint(0, 32, (20 + i % 9,), generator=g).tolist() for i in range(60)]
+        # every fourth request of the second engine draws at random between the others
+        heat = [dict(temperature=5.0) if i % 4 == 3 else settings for i in range(60)]
+        a = [one.submit(p, 60) for p in prompts]
+        b = [eng.submit(p, 60, **s) for p, s in zip(prompts, heat)]
+        for e, rr in ((one, a), (eng, b)):
+            while any(not e._requests[r].generated for r in rr):
+                e.step()
+        # the model's own texts, a token a call
+        seen, texts, leads = watch(one), [[] for _ in a], []
+        for _ in range(4):
+            got = one.step_drafts({r: ([], []) for r in a})
+            leads.append(lead(seen[-1]))
+            for text, r in zip(texts, a):
+                text += got[r]
+        least = torch.stack(leads).amin(0).tolist()
+        # drafts in 16 bits where the first engine read them in 8: 3 keys of 20 or more
+        sd = SD + (2 * 2.0 ** -4 * math.sqrt(1 / 3) * 3 / 20 if kw.get("kv_fp8") else 0)
+        sure = [i for i in range(60) if i % 4 != 3 and least[i] > 4 * math.sqrt(2) * sd
+                and one._requests[a[i]].generated[:-4] == eng._requests[b[i]].generated]
+        assert len(sure) >= 2
+        before = {i: list(eng._requests[b[i]].generated) for i in sure}
+        # right ones behind wrong ones beside them, and wrong ones below
+        drafts = {}
+        for i, r in enumerate(b):
+            c1, c2, c3, _ = texts[i]
+            drafts[r] = ([(c1 + 1) % 32, c1, (c2 + 1) % 32, c2, c1, (c3 + 3) % 32, c3], [-1, -1, 1, 1, 0, 3, 3])
+        got = eng.step_drafts(drafts)
+        for i in sure:
+            req, rid = eng._requests[b[i]], b[i]
+            assert got[rid] == texts[i] and req.generated == before[i] + texts[i]
+            tokens = prompts[i] + req.generated[:-1]
+            assert eng.seq_len[req.slot].item() == eng._seq_len_host[req.slot] == len(tokens)
+            assert eng._last_tok[req.slot].item() == texts[i][-1]
+            ref = engine(vocab_size=32, **kw)
+            rr = ref.submit(tokens, 2)
+            ref.step()
+            x, y = kv_rows(eng, req.slot, len(tokens)), kv_rows(ref, ref._requests[rr].slot, len(tokens))
+            # a K that is rotated by one position too few is off by about its own size
+            assert (x - y).abs().max() <= (0.3 if kw.get("kv_fp8") else 0.06) * max(1.0, y.abs().max().item())
+            if not kw.get("kv_fp8"):
+                # row by row, what layers of 12 roundings leave
+                assert ((x - y).norm(dim=-1) <= 12 * HALF * y.norm(dim=-1)).all()
