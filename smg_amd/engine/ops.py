@@ -100,11 +100,16 @@ def _scale(scale: Optional[float], D: int) -> float:
     return scale
 
 
+def _repeats(t: torch.Tensor) -> bool:
+    """Whether several of its elements share a place in memory by a stride of 0."""
+    return 0 in t.stride() and any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape))
+
+
 def _out(out: Optional[torch.Tensor], q: torch.Tensor, dev: int) -> torch.Tensor:
     if out is None:
         return torch.empty_like(q, memory_format=torch.contiguous_format)
     _check("out", out, (_BF16,), q.dim(), dev)
-    if out.shape != q.shape or 0 in out.stride():
+    if out.shape != q.shape or _repeats(out):
         raise ValueError(f"out must be {tuple(q.shape)} with a place for every element, got {tuple(out.shape)} with strides {out.stride()}")
     return out
 
@@ -193,8 +198,9 @@ def attn_prefill(
 
     max_ctx, a bound on starts[b] plus the new tokens, only sizes the split of
     long caches over the card (default: the cache's length).  Returns out
-    [N, H, D], which may be q itself; rows that no sequence covers are not written.  A sequence whose slot
-    lies outside the cache gets zeros."""
+    [N, H, D], which may be q itself and shares no memory with the arguments otherwise;
+    rows that no sequence covers are not written.  A sequence whose slot lies outside
+    the cache gets zeros."""
     _check("q", q, (_BF16,), 3, None)
     dev = q.get_device()
     N, H, D = q.shape
@@ -237,7 +243,8 @@ def attn_tree(
     sequence whose slot lies outside the cache.
 
     max_ctx, a bound on ctx_lens, only sizes the split of long caches over the
-    card (default: the cache's length).  Returns out [B, N, H, D], which may be q."""
+    card (default: the cache's length).  Returns out [B, N, H, D], which may be q
+    itself and shares no memory with the arguments otherwise."""
     _check("q", q, (_BF16,), 4, None)
     dev = q.get_device()
     B, N, H, D = q.shape
@@ -300,7 +307,7 @@ def tree_commit(
         raise ValueError(f"head dim must be a multiple of 8, got {D}")
     if B > MAX_SEQUENCES:
         raise ValueError(f"at most {MAX_SEQUENCES} sequences, got {B}")
-    if 0 in kv_cache.stride():
+    if _repeats(kv_cache):
         raise ValueError(f"kv_cache must have a place for every element, strides {kv_cache.stride()}")
     if N > MAX_NODES or (N < 1 and B > 0):
         raise ValueError(f"1 to {MAX_NODES} drafted nodes, got {N}")

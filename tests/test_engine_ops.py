@@ -820,6 +820,16 @@ class TestRefusals:
             getattr(self, call)(**kw)
 
 
+    def test_a_stride_of_one_element_does_not_matter(self):
+        """Nothing but the device is wrong with these."""
+        one = lambda *shape: torch.zeros(4096, dtype=BF16).as_strided(shape, (0, *torch.zeros(shape[1:]).stride()))  # noqa: E731
+        cu = torch.tensor([0, 1], dtype=torch.int32)
+        zero = torch.zeros(1, dtype=torch.int32)
+        for call in (lambda: self.prefill(q=one(1, 4, 64), out=one(1, 4, 64), slots=zero, starts=zero, cu=cu),
+                     lambda: self.commit(kn=torch.zeros(1, 2, 2, 3, 1, 8, dtype=BF16), kv=one(1, 2, 4, 1, 16, 8))):
+            with pytest.raises(RuntimeError, match="CUDA/HIP"):
+                call()
+
     @pytest.mark.parametrize("call,name,shape,dtype", [
         ("prefill", "q", (6, 4, 64), BF16), ("prefill", "k", (2, 2, 16, 64), BF16), ("prefill", "v", (2, 2, 16, 64), BF16),
         ("prefill", "out", (6, 4, 64), BF16), ("tree", "q", (2, 3, 4, 64), BF16), ("tree", "kn", (2, 3, 2, 64), BF16),
