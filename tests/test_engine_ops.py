@@ -1364,3 +1364,24 @@ class TestEngineAnswers:
             if not kw.get("kv_fp8"):
                 # row by row, what layers of 12 roundings leave
                 assert ((x - y).norm(dim=-1) <= 12 * HALF * y.norm(dim=-1)).all()
+
+
+@pytest.mark.gpu
+def test_a_sampled_request_between_captured_forwards():
+    """Captured forwards end in an argmax: a sampled request takes the others out of them and
+    back, and changes none of their tokens."""
+    from smg_amd.engine.torch_engine import TorchEngine
+
+    outs = []
+    for graphs in (False, True):
+        eng = TorchEngine(engine("cpu").cfg, device=DEV, graphs=graphs)
+        texts = []
+        for wave in range(5):  # equal groups, so that prefill is captured too
+            greedy = [eng.submit([(wave * 50 + i * 9 + j) % 2048 for j in range(40)], 12) for i in range(4)]
+            if wave in (1, 3, 4):
+                sampled = eng.submit(list(range(7)), 5, temperature=1.0, top_p=0.9)
+            texts += run(eng, *greedy)
+        assert eng.finished(sampled)
+        assert bool(eng._graph_cache) == graphs
+        outs.append(texts)
+    assert outs[0] == outs[1]
