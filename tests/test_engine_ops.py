@@ -866,6 +866,16 @@ class TestTogether:
         assert [t.numel() for t in got] == [0, 0, 0]
         assert ops.sample(e(0, 5), e(0, d=torch.float32), e(0, d=torch.float32)).numel() == 0
 
+    @pytest.mark.parametrize("fp8", [False, True])
+    def test_same_bits_every_time(self, fp8):
+        cases = [(ops.attn_prefill, prefill_case(lens, starts, 8, 2, 128, fp8, seed=13))
+                 for lens, starts in (([300, 1, 77], [0, 5, 64]), ([3, 40], [6000, 900]))]
+        cases += [(ops.attn_tree, tree_case(len(ctx), 33, ctx, 8, 2, 128, fp8, seed=14)) for ctx in ([700] * 40, [9000, 3])]
+        for call, args in cases:
+            first = call(*args)
+            for _ in range(5):
+                assert torch.equal(first.view(torch.int16), call(*args).view(torch.int16))
+
     def test_on_another_stream(self):
         s = torch.cuda.Stream()
         pre, tre = prefill_case([9, 70], [3000, 4], 8, 2, 128, seed=1), tree_case(2, 9, [2500, 7], 8, 2, 128, seed=2)
