@@ -205,7 +205,8 @@ def execute_transfers(engine, transfers) -> int:
     """Run one tick's ordered PD KV handoffs against the local engine.
     Entries: (rid, peer, direction, n_tokens, first_tok, max_new).  Both
     endpoints iterate the SAME list, so sends and recvs pair in order; fp8
-    caches travel as uint8 views (NCCL has no fp8 dtype)."""
+    caches travel as uint8 views (NCCL has no fp8 dtype).  Sampling settings
+    are no part of an entry: a request that sampled goes on greedily."""
     tag = KV_TAG if dist.get_backend() == "gloo" else 0
     done = 0
     for rid, peer, direction, n_tokens, first_tok, max_new in transfers:

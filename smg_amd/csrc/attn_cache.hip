@@ -32,14 +32,15 @@
 //   16384 tokens, 16 over 4 heads of 128: 1.10 ms, 1.00 PF/s.  Matrix cores
 //     are busy 54% of the cycles and the vector unit, with exp and the
 //     roundings, 56%; under both the clock falls to 1.9 GHz.
-//   two chunks of 1900 tokens over 5900 8-bit rows, 16 heads: 273 us, 0.79 PF/s.
+//   two chunks of 1900 tokens over 5900 8-bit rows, 16 heads: 270 us, 0.80 PF/s.
 //     One workgroup of 8 waves a compute unit where 16 bits have two of 4, and
 //     7% for the widening.
-//   32 prompts of about 75 over 460 rows: 31 us; half of the units have two
-//     workgroups and the others one.
-//   64 trees of 16 nodes over 1150 rows: 51 us, 3.2 TB/s of K/V, 38 where the
-//     caches hold them: one tile's latency after the other.
-//   4 trees of 61 over 35000 8-bit rows: 106 us, of which joining takes 9.
+//   32 prompts of about 75 over 460 rows: 30 us; 104 of the units have two
+//     workgroups and 152 one, and 19% of the rows computed are padding.
+//   64 trees of 16 nodes over 250 to 2000 rows: 51 us, 3.2 TB/s of K/V, 38 where
+//     the caches hold them.  Each unit has one workgroup and its whole sequence:
+//     the longest take 17 tiles of keys, the mean one 10.6.
+//   4 trees of 61 over 35000 8-bit rows: 106 us, of which joining takes 10.
 //   one prompt of a token, or a tree of 5: 6.5 and 7.5 us, latency alone.
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>
@@ -190,8 +191,10 @@ __device__ __forceinline__ void add_where(f32x16& acc, u32x4 v, bf16x8 p, float 
 }
 
 // Tiles hold D bf16 a row in 16-byte chunks, permuted within the row so that
-// the reads below touch every bank once: 8 lanes reading one chunk column of 8
-// key rows (K), and 4 rows of 32 bytes, a pair of chunks (V).
+// neighbouring lanes read different banks: 8 lanes one chunk column of 8 key
+// rows (K), and 4 rows of 32 bytes, a pair of chunks (V).  The counters still
+// have 33% of the LDS cycles as conflicts (36% in 8 bits); which of the reads or
+// DMA writes they come from has not been told apart.
 template <int D>
 __device__ __forceinline__ int k_chunk(int row, int c) {
     return row * (D / 8) + (c ^ (row & (D / 8 - 1)));
@@ -323,8 +326,9 @@ struct Tile {
 // WR waves share the query rows of a tile (32 each), WK of them split its keys:
 // 4 x 1 reads K/V least often, 2 x 2 makes twice the workgroups, 2 x 4 and 1 x 4 have
 // twice the bytes on their way from a compute unit that has one workgroup.  A wave takes
-// 64 keys of a tile, or 32 where waves split it, as one block hides less latency than two
-// but leaves registers for two workgroups (64 trees of 16 nodes: 51 us, 59 with 64).
+// 64 keys of a tile, or 32 where waves split it: so 2 x 2 takes 64 KB of LDS and a compute
+// unit two workgroups of it (24 prompts of 75 over 460 rows: 22 us, 34 with 64 keys and one
+// workgroup; one prompt of 2048: 39 and 43), and 2 x 4, with 128 KB of tiles, fits at all.
 template <bool TREE, bool KV8, int D, int WR, int WK_>
 struct Shape {
     static constexpr int WK = WK_;

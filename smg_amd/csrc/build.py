@@ -42,8 +42,8 @@ def build(verbose: bool = True, force: bool = False) -> Path:
         "-fPIC",
         "-shared",
         "-fvisibility=hidden",
-        # packed f32 arithmetic is left out: some of its forms have given wrong
-        # results on gfx950 now and then
+        # no packed f32 arithmetic in any of the sources: some of its forms are
+        # known to be unreliable on these cards
         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
         "-parallel-jobs=8",
         f"-I{pybind11.get_include()}",

@@ -153,6 +153,12 @@ def _shape(total: int, each: int, B: int, KVH: int, D: int, fp8: bool, ctx: int)
     heads: 21 us with 2 waves, 24 with 4, 37 with 1; 32 of them: 34, 32 and 63).  Where each
     workgroup has a compute unit for itself, more waves take its keys (64 trees of 16 nodes
     over 1150 rows: 38 us by 2 x 4 waves, 43 by 2 x 2; with twice the workgroups 43 and 34).
+    4 waves along the rows pay in 16 bits where that leaves more workgroups than units by far
+    (24 prompts, 260 workgroups: 25 us, 22 by 2; 32, 356: 30 and 32; one prompt of 3000
+    tokens with 372 loses all the same: 73 and 56).  In 8 bits a unit takes one workgroup: 2
+    waves until there are more of them than units (12 prompts, 124 of 4: 24 us by 2, 26 by 4;
+    16, 176 of 4: 39 and 26), 8 where 4 would be more (32 prompts, 208 of 8: 34 us, 46 by 4;
+    one of 3000, 184 of 8: 103 and 82).
     Splitting keys fills the card with few rows, and writes and reads partial results of as
     many rows as it takes at once: it has to save the time of about 1450 keys in 16 bits,
     650 in 8 (8 trees of 61 nodes over up to 4000 rows: 41 us split, 53 not; 16 prompts of 18
@@ -161,17 +167,18 @@ def _shape(total: int, each: int, B: int, KVH: int, D: int, fp8: bool, ctx: int)
         at_once = 32 * waves
         return KVH * (B * -(-each // at_once) if each else max(B, total // at_once + B // 2))
 
+    units = 256  # compute units
     long = total > 128 * B and ctx >= 4096  # rows for 8 waves, and K/V worth reading once
     runs = max(1, min(64, ctx // 256))
     if fp8:
         four = work(4)
-        if ctx * (256 - four) > 650 * 256:
+        if ctx * (units - four) > 650 * units:
             return (8, 1, runs) if long else (4, 2, runs)
         return (8, 1, 1) if total > 128 * B and work(8) >= 200 else (4, 2, 1) if four >= 100 else (2, 2, 1)
     two = work(2)
-    if ctx * (256 - two) > 1450 * 256:
+    if ctx * (units - two) > 1450 * units:
         return (4, 1, runs) if long else (2, 2, runs)
-    if D == 128 and two <= 256:
+    if D == 128 and two <= units:
         return (1, 4, 1) if two <= 64 else (2, 4, 1)
     return (4, 1, 1) if total > 64 * B and work(4) >= 320 else (2, 2, 1)
 

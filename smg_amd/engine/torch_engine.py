@@ -60,8 +60,10 @@ class TorchEngineConfig:
     kv_fp8: bool = False
     # opt-in packed prefill: prompts and chunks of different lengths and
     # histories share one forward (ops.attn_prefill) instead of waiting for
-    # others of their length (32 prompts of 40 to 400 tokens: 22 ms, 224
-    # without).  Requires the gfx950 kernels.
+    # others of their length (32 prompts of 40 to 400 tokens: 23 ms, 213
+    # without).  With kv_fp8 a prompt's tokens see each other's K/V in 8 bits
+    # too, as decoding does; the batched prefill reads those of the chunk in
+    # 16.  Requires the gfx950 kernels.
     packed_prefill: bool = False
 
     @classmethod
@@ -415,7 +417,9 @@ class TorchEngine:
 
         `temperature` above 0 samples the request's tokens (ops.sample) with
         `top_k` (0: all), `top_p` (1: all) and `min_p` (0: none) from the
-        engine's own generator; 0 takes the likeliest token."""
+        engine's own generator; 0 takes the likeliest token.  The settings stay
+        with this engine: import_kv() on another takes them as its arguments,
+        and a handoff over the plane, which carries none, goes on greedily."""
         sampling = self._sampling_settings(temperature, top_k, top_p, min_p)
         if rid is None:
             self._rid_counter += 1
