@@ -818,7 +818,7 @@ class TorchEngine:
         pin, dev, copied = entry
         pin[:n].numpy()[:] = arr
         dev[:n].copy_(pin[:n], non_blocking=True)
-        copied.record()
+        copied.record(torch.cuda.current_stream(self.device))
         return dev[:n]
 
     def _get_slab(self, n: int) -> torch.Tensor:

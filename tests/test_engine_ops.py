@@ -1191,7 +1191,8 @@ class TestStaging:
             del stream[:n]
 
         class Event:
-            def record(self):
+            def record(self, at):
+                assert at == ("stream of", torch.device(DEV))  # the copy's, whatever device is current
                 self.place = len(ran) + len(stream)
 
             def synchronize(self):
@@ -1212,6 +1213,7 @@ class TestStaging:
         eng.device = torch.device(DEV)
         monkeypatch.setattr(torch, "empty", cpu_empty)
         monkeypatch.setattr(torch.cuda, "Event", Event)
+        monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: ("stream of", device))
         sent = [[i] * (1 + i % 5) for i in range(3 * len(eng._h2d_bufs))]
         for values in sent:
             eng._h2d_i64(values)
